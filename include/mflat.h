@@ -23,6 +23,7 @@
 #ifndef MFLAT_H
 #define MFLAT_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #if defined(_WIN32)
@@ -233,6 +234,129 @@ MFLAT_API mflat_status_t mflat_coarse_set_shard(mflat_coarse_t*, int rank, int w
 MFLAT_API mflat_status_t mflat_flat_save(const mflat_flat_index_t*, const char* path);
 MFLAT_API mflat_flat_index_t* mflat_flat_load(const char* path, int device,
                                               mflat_status_t* out_status);
+
+/* ---------------- Selection operators of language models -------------- */
+/* ADDITIVE (no counterpart in the reference).  The library's selection -- the
+ * k best scores, ties to the lowest id, -1 padding where fewer exist -- for the
+ * three places where a model that runs beside an index selects at every token:
+ * routing to experts, beam search, eviction from a key/value cache.
+ *
+ * Every pointer is device memory on `device` (-1 = MFLAT_DEVICE or 0) and every
+ * call only enqueues on `stream` (a cudaStream_t, NULL = the legacy default
+ * stream): no allocation, no host synchronisation, so calls can be captured
+ * into CUDA graphs.  Scratch is the caller's `workspace` (256-byte aligned, the
+ * size from *_workspace_bytes, no initial contents needed): calls that may
+ * overlap on the GPU, and captured graphs that may, need one each.  Strides are
+ * in elements unless they say bytes; 0 stands for densely packed rows.
+ * A missing pointer -> NULL_ARG; a size, type or stride outside the stated
+ * limits, a misaligned pointer (less than its element's size) or a workspace
+ * too small -> BAD_ARG with a line in the log; CUDA failure -> DEVICE. */
+#define MFLAT_ROUTE_MAX_EXPERTS 1024
+#define MFLAT_ROUTE_MAX_K 32
+#define MFLAT_ROUTE_MAX_GROUPS 32
+#define MFLAT_BEAM_MAX_BEAMS 64
+#define MFLAT_BEAM_MAX_K 128
+
+typedef enum {
+    MFLAT_SCORE_SOFTMAX = 0,
+    MFLAT_SCORE_SIGMOID = 1
+} mflat_score_t;
+
+/* A router over `experts` experts.  Scores s = softmax(x) or sigmoid(x) of a
+ * token's logits x; the choice goes by c = s + bias (bias given) or by x, the k
+ * largest first, ties to the lowest expert.  Logits of -inf or NaN (and biases
+ * of -inf or NaN) are never chosen and weigh nothing.  groups > 1: the experts
+ * form that many groups of adjacent ones, a group's score is the sum of its
+ * group_top (1 or 2) largest s + bias, and only the groups_kept best groups
+ * take part.  Weights are s of the chosen (without bias), divided by their sum
+ * where `renormalise` is set, times `scale`. */
+typedef struct {
+    int experts, k;                 /* 1..MAX_EXPERTS; 1..min(MAX_K, experts)       */
+    mflat_score_t score;
+    mflat_storage_t type;           /* of the logits                                */
+    int renormalise;
+    int groups, groups_kept;        /* groups divides experts, 1..MAX_GROUPS        */
+    int group_top;                  /* 1 or 2                                       */
+    float scale;
+} mflat_router_t;
+
+/* Scratch of the lists by expert (0: none needed, or an invalid router). */
+MFLAT_API size_t mflat_route_workspace_bytes(const mflat_router_t*, int tokens);
+/* d_out_ids / d_out_weights: tokens x k, -1 / 0 padded.  d_mask (nullable):
+ * tokens with 0 are padding, ids -1 and weights 0.  d_out_start (experts + 1)
+ * and d_out_slots (tokens x k), both or neither: the CSR lists by expert --
+ * entries t * k + j with id e, ascending, at [start[e], start[e + 1]); slots
+ * behind start[experts] are left as they were. */
+MFLAT_API mflat_status_t mflat_route_device(const mflat_router_t*, const void* d_logits,
+        int64_t stride, int tokens, const float* d_bias, const uint8_t* d_mask,
+        int32_t* d_out_ids, float* d_out_weights, int32_t* d_out_start, int32_t* d_out_slots,
+        void* d_workspace, size_t workspace_bytes, int device, void* stream);
+/* Gradient of the logits (their type, every expert written) from the gradient
+ * of the weights (fp32, tokens x k) of the choice in d_ids.  Entries of d_ids
+ * outside [0, experts) carry no gradient; a repeated one adds up.  The choice
+ * itself and the bias have none.  d_out_grad may be d_logits (same stride). */
+MFLAT_API mflat_status_t mflat_route_backward_device(const mflat_router_t*, const void* d_logits,
+        int64_t stride, int tokens, const int32_t* d_ids, const float* d_grad_weights,
+        void* d_out_grad, int64_t grad_stride, int device, void* stream);
+
+/* A beam search step over beams x vocabulary.  key = cum + log softmax(x)[v],
+ * compared in 64 bits; the k largest of a sequence's beams * vocab, ties to the
+ * lowest beam, then token.  A finished beam proposes only (eos, cum); logits of
+ * -inf or NaN, and beams whose cum is not finite, propose nothing. */
+typedef struct {
+    int beams, vocab, k;            /* 1..MAX_BEAMS; >= 1; 1..MAX_K                 */
+    mflat_storage_t type;           /* of the logits                                */
+    int eos;                        /* token of finished beams, -1 = none finish    */
+} mflat_beam_t;
+
+MFLAT_API size_t mflat_beam_workspace_bytes(const mflat_beam_t*, int batch);
+/* d_logits: (batch * beams) rows of vocab; d_cum, d_finished (nullable): batch x
+ * beams.  Outputs batch x k: parent beam, token, new cum; -1 / -1 / -inf padded. */
+MFLAT_API mflat_status_t mflat_beam_select_device(const mflat_beam_t*, const void* d_logits,
+        int64_t stride, const float* d_cum, const uint8_t* d_finished, int batch,
+        int32_t* d_out_parents, int32_t* d_out_tokens, float* d_out_scores,
+        void* d_workspace, size_t workspace_bytes, int device, void* stream);
+/* Reorders states in place: row (o, b, i) becomes what row (o, b, parent[b][i])
+ * was, for every o < outer, b < batch, i < beams.  A row is `segments` pieces of
+ * segment_bytes, segment_stride apart; strides in BYTES (0: dense), d_parents
+ * rows parent_stride apart (0: beams).  Parents outside [0, beams) leave their
+ * row alone; bytes between the pieces are not touched. */
+MFLAT_API mflat_status_t mflat_beam_reorder_device(void* d_states, const int32_t* d_parents,
+        int64_t parent_stride, int outer, int batch, int beams, int segments,
+        int64_t segment_bytes, int64_t segment_stride, int64_t row_stride, int64_t outer_stride,
+        int device, void* stream);
+
+/* Eviction from a key/value cache by accumulated attention weight.  Per
+ * sequence b and cache head h: acc' = acc + the weights of the group's query
+ * heads and query rows, rounded once to fp32.  With more than `budget` entries
+ * the kept ones are those at positions < sink or >= seen[b] - recent (equals),
+ * then the largest acc', ties to the lowest slot (NaN last).  The i-th free slot below
+ * `budget` takes the i-th kept entry behind it: few rows move, slots lose the
+ * positions' order, d_pos tells them. */
+typedef struct {
+    int heads, group;               /* cache heads; query heads per cache head      */
+    int capacity;                   /* slots per (sequence, head)                   */
+    int budget, recent, sink;       /* sink + recent <= budget <= capacity          */
+    mflat_storage_t type;           /* of the attention weights                     */
+    int64_t key_bytes, value_bytes; /* one entry's row; 0 = no such buffer          */
+    int64_t key_stride[3];          /* BYTES from sequence / head / slot to the     */
+    int64_t value_stride[3];        /* next; all 0 = dense [b][h][slot]             */
+} mflat_cache_t;
+
+MFLAT_API size_t mflat_cache_workspace_bytes(const mflat_cache_t*, int batch);
+/* d_lens, d_seen: batch (entries held; tokens seen so far).  d_weights (nullable:
+ * nothing to add): [b][heads * group][queries][slot], strides in elements from
+ * sequence / head / query row to the next (NULL: rows of `capacity`); only slots
+ * below the length are read.  d_rows (nullable): batch, valid query rows.  d_acc,
+ * d_pos: batch x heads x capacity; outputs may be the same buffers.  Slots
+ * behind the new length are left as they were in every output.  d_out_lens
+ * (batch) must not be d_lens. */
+MFLAT_API mflat_status_t mflat_cache_evict_device(const mflat_cache_t*, int batch,
+        const int32_t* d_lens, const int32_t* d_seen, const void* d_weights, int queries,
+        const int64_t weight_stride[3], const int32_t* d_rows, const float* d_acc,
+        const int32_t* d_pos, float* d_out_acc, int32_t* d_out_pos, int32_t* d_out_lens,
+        void* d_keys, void* d_values, void* d_workspace, size_t workspace_bytes, int device,
+        void* stream);
 
 #ifdef __cplusplus
 }

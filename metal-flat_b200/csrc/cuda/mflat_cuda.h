@@ -10,6 +10,7 @@
 #ifndef MFLAT_CUDA_H
 #define MFLAT_CUDA_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #if defined(_WIN32)
@@ -124,6 +125,49 @@ MFLAT_CU_API const int32_t* mflat_cu_kmeans_reordered_device(const mflat_cu_kmea
 MFLAT_CU_API int mflat_cu_comm_unique_id(uint8_t* out_id /* 128 bytes */);
 MFLAT_CU_API int mflat_cu_index_set_shard(mflat_cu_index_t* ix, int rank, int world,
                                           const uint8_t* comm_id, int64_t id_base);
+
+/* Selection operators (route.cu, beam.cu, cache.cu): the structures and rules of
+ * include/mflat.h's mflat_route_*, mflat_beam_* and mflat_cache_* entries.  Every
+ * pointer is device memory, the calls only enqueue on `stream`. */
+typedef struct {
+    int experts, k, score, type, renormalise, groups, groups_kept, group_top;
+    float scale;
+} mflat_cu_router_t;
+MFLAT_CU_API size_t mflat_cu_route_workspace(const mflat_cu_router_t* r, int tokens);
+MFLAT_CU_API int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, int64_t stride,
+                                int tokens, const float* bias, const uint8_t* mask, int32_t* ids,
+                                float* weights, int32_t* start, int32_t* slots, void* ws,
+                                size_t ws_bytes, int device, void* stream);
+MFLAT_CU_API int mflat_cu_route_backward(const mflat_cu_router_t* r, const void* logits,
+                                         int64_t stride, int tokens, const int32_t* ids,
+                                         const float* grad_weights, void* grad, int64_t grad_stride,
+                                         int device, void* stream);
+
+typedef struct {
+    int beams, vocab, k, type, eos;
+} mflat_cu_beam_t;
+MFLAT_CU_API size_t mflat_cu_beam_workspace(const mflat_cu_beam_t* b, int batch);
+MFLAT_CU_API int mflat_cu_beam_select(const mflat_cu_beam_t* b, const void* logits, int64_t stride,
+                                      const float* cum, const uint8_t* finished, int batch,
+                                      int32_t* parents, int32_t* tokens, float* scores, void* ws,
+                                      size_t ws_bytes, int device, void* stream);
+MFLAT_CU_API int mflat_cu_beam_reorder(void* states, const int32_t* parents, int64_t parent_stride,
+                                       int outer, int batch, int beams, int segments,
+                                       int64_t segment_bytes, int64_t segment_stride,
+                                       int64_t row_stride, int64_t outer_stride, int device,
+                                       void* stream);
+
+typedef struct {
+    int heads, group, capacity, budget, recent, sink, type;
+    int64_t key_bytes, value_bytes, key_stride[3], value_stride[3];
+} mflat_cu_cache_t;
+MFLAT_CU_API size_t mflat_cu_cache_workspace(const mflat_cu_cache_t* c, int batch);
+MFLAT_CU_API int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const int32_t* lens,
+                                      const int32_t* seen, const void* weights, int queries,
+                                      const int64_t* weight_stride, const int32_t* rows,
+                                      const float* acc, const int32_t* pos, float* out_acc,
+                                      int32_t* out_pos, int32_t* out_lens, void* keys, void* values,
+                                      void* ws, size_t ws_bytes, int device, void* stream);
 
 #ifdef __cplusplus
 }

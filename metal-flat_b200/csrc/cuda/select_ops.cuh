@@ -1,0 +1,75 @@
+// select_ops.cuh -- what the selection operators (route.cu, beam.cu, cache.cu)
+// share: element types, order-preserving keys, argument checks and launches.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "index_impl.cuh"
+
+namespace mflat_cu {
+
+constexpr unsigned kFullMask = 0xffffffffu;
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <class T>
+__device__ __forceinline__ T from_float(float v) {
+    if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+    else return v;
+}
+
+// N elements as one aligned load or store of N * sizeof(T) bytes.
+template <class T, int N>
+struct alignas(N * sizeof(T)) Pack {
+    T v[N];
+};
+
+// Keys whose order is the value's, for selection by integer comparison.
+// Equal values (-0 and +0 among them) get equal keys; 0 is left for "no
+// candidate", which NaN and -inf map to: a selection never takes them.
+__device__ __forceinline__ uint32_t choice_key(float v) {
+    if (!(v > neg_inf())) return 0u;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t choice_key(double v) {
+    if (!(v > static_cast<double>(neg_inf()))) return 0ull;
+    const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+    return (u >> 63) ? ~u : (u | (1ull << 63));
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    if (k == 0u) return neg_inf();
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ double key_value(uint64_t k) {
+    if (k == 0ull) return static_cast<double>(neg_inf());
+    return __longlong_as_double(static_cast<long long>((k >> 63) ? (k & ~(1ull << 63)) : ~k));
+}
+
+inline size_t type_bytes(int type) { return type == 0 ? 4 : 2; }
+inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
+
+// Device of a call: resolved and present, or a status with its message.
+int operator_device(int device, int* out);
+
+// Calls fn with a value of the element type that `type` (mflat_storage_t) names.
+template <class Fn>
+cudaError_t with_type(int type, Fn&& fn) {
+    switch (type) {
+        case 0: return fn(float{});
+        case 1: return fn(__half{});
+        default: return fn(__nv_bfloat16{});
+    }
+}
+
+}  // namespace mflat_cu

@@ -16,6 +16,7 @@
 
 #include "../../../include/mflat.h"
 #include "../cuda/mflat_cuda.h"
+#include "Log_internal.h"
 #include "metalflat/CoarseQuantizer.h"
 #include "metalflat/FlatIndex.h"
 #include "metalflat/Log.h"
@@ -87,6 +88,28 @@ mflat_status_t from_cu(int st) {
         case 5: return MFLAT_ERR_INTERNAL;
         default: return MFLAT_ERR_DEVICE;
     }
+}
+
+// Status of a selection operator's call; a refusal or failure says why in the log.
+mflat_status_t reported(int st, const char* op) {
+    if (st != 0) MFLAT_LOG_ERROR("%s: %s", op, mflat_cu_last_error());
+    return from_cu(st);
+}
+
+mflat_cu_router_t to_cu(const mflat_router_t& r) {
+    return {r.experts, r.k, static_cast<int>(r.score), static_cast<int>(r.type), r.renormalise,
+            r.groups, r.groups_kept, r.group_top, r.scale};
+}
+
+mflat_cu_beam_t to_cu(const mflat_beam_t& b) {
+    return {b.beams, b.vocab, b.k, static_cast<int>(b.type), b.eos};
+}
+
+mflat_cu_cache_t to_cu(const mflat_cache_t& c) {
+    return {c.heads, c.group, c.capacity, c.budget, c.recent, c.sink, static_cast<int>(c.type),
+            c.key_bytes, c.value_bytes,
+            {c.key_stride[0], c.key_stride[1], c.key_stride[2]},
+            {c.value_stride[0], c.value_stride[1], c.value_stride[2]}};
 }
 
 }  // namespace
@@ -429,6 +452,101 @@ MFLAT_API mflat_flat_index_t* mflat_flat_load(const char* path, int device, mfla
     }
     if (st) *st = rc;
     return h;
+}
+
+MFLAT_API size_t mflat_route_workspace_bytes(const mflat_router_t* r, int tokens) {
+    if (!r) return 0;
+    const mflat_cu_router_t c = to_cu(*r);
+    return mflat_cu_route_workspace(&c, tokens);
+}
+
+MFLAT_API mflat_status_t mflat_route_device(const mflat_router_t* r, const void* logits,
+                                            int64_t stride, int tokens, const float* bias,
+                                            const uint8_t* mask, int32_t* ids, float* weights,
+                                            int32_t* start, int32_t* slots, void* ws,
+                                            size_t ws_bytes, int device, void* stream) {
+    if (!r || (tokens > 0 && (!logits || !ids || !weights))) return MFLAT_ERR_NULL_ARG;
+    if (!start != !slots && (tokens > 0 || !start)) return MFLAT_ERR_NULL_ARG;
+    return guarded([&] {
+        const mflat_cu_router_t c = to_cu(*r);
+        return reported(mflat_cu_route(&c, logits, stride, tokens, bias, mask, ids, weights, start,
+                                       slots, ws, ws_bytes, device, stream),
+                        "route");
+    });
+}
+
+MFLAT_API mflat_status_t mflat_route_backward_device(const mflat_router_t* r, const void* logits,
+                                                     int64_t stride, int tokens, const int32_t* ids,
+                                                     const float* grad_weights, void* grad,
+                                                     int64_t grad_stride, int device, void* stream) {
+    if (!r || (tokens > 0 && (!logits || !ids || !grad_weights || !grad))) return MFLAT_ERR_NULL_ARG;
+    return guarded([&] {
+        const mflat_cu_router_t c = to_cu(*r);
+        return reported(mflat_cu_route_backward(&c, logits, stride, tokens, ids, grad_weights, grad,
+                                                grad_stride, device, stream),
+                        "route backward");
+    });
+}
+
+MFLAT_API size_t mflat_beam_workspace_bytes(const mflat_beam_t* b, int batch) {
+    if (!b) return 0;
+    const mflat_cu_beam_t c = to_cu(*b);
+    return mflat_cu_beam_workspace(&c, batch);
+}
+
+MFLAT_API mflat_status_t mflat_beam_select_device(const mflat_beam_t* b, const void* logits,
+                                                  int64_t stride, const float* cum,
+                                                  const uint8_t* finished, int batch,
+                                                  int32_t* parents, int32_t* tokens, float* scores,
+                                                  void* ws, size_t ws_bytes, int device,
+                                                  void* stream) {
+    if (!b || (batch > 0 && (!logits || !cum || !parents || !tokens || !scores)))
+        return MFLAT_ERR_NULL_ARG;
+    return guarded([&] {
+        const mflat_cu_beam_t c = to_cu(*b);
+        return reported(mflat_cu_beam_select(&c, logits, stride, cum, finished, batch, parents,
+                                             tokens, scores, ws, ws_bytes, device, stream),
+                        "beam select");
+    });
+}
+
+MFLAT_API mflat_status_t mflat_beam_reorder_device(void* states, const int32_t* parents,
+                                                   int64_t parent_stride, int outer, int batch,
+                                                   int beams, int segments, int64_t segment_bytes,
+                                                   int64_t segment_stride, int64_t row_stride,
+                                                   int64_t outer_stride, int device, void* stream) {
+    if (outer > 0 && batch > 0 && segments > 0 && segment_bytes > 0 && (!states || !parents))
+        return MFLAT_ERR_NULL_ARG;
+    return guarded([&] {
+        return reported(mflat_cu_beam_reorder(states, parents, parent_stride, outer, batch, beams,
+                                              segments, segment_bytes, segment_stride, row_stride,
+                                              outer_stride, device, stream),
+                        "beam reorder");
+    });
+}
+
+MFLAT_API size_t mflat_cache_workspace_bytes(const mflat_cache_t* c, int batch) {
+    if (!c) return 0;
+    const mflat_cu_cache_t u = to_cu(*c);
+    return mflat_cu_cache_workspace(&u, batch);
+}
+
+MFLAT_API mflat_status_t mflat_cache_evict_device(
+    const mflat_cache_t* c, int batch, const int32_t* lens, const int32_t* seen,
+    const void* weights, int queries, const int64_t weight_stride[3], const int32_t* rows,
+    const float* acc, const int32_t* pos, float* out_acc, int32_t* out_pos, int32_t* out_lens,
+    void* keys, void* values, void* ws, size_t ws_bytes, int device, void* stream) {
+    if (!c || (batch > 0 && (!lens || !seen || !acc || !pos || !out_acc || !out_pos || !out_lens)))
+        return MFLAT_ERR_NULL_ARG;
+    if (batch > 0 && ((c->key_bytes > 0 && !keys) || (c->value_bytes > 0 && !values)))
+        return MFLAT_ERR_NULL_ARG;
+    return guarded([&] {
+        const mflat_cu_cache_t u = to_cu(*c);
+        return reported(mflat_cu_cache_evict(&u, batch, lens, seen, weights, queries, weight_stride,
+                                             rows, acc, pos, out_acc, out_pos, out_lens, keys,
+                                             values, ws, ws_bytes, device, stream),
+                        "cache evict");
+    });
 }
 
 }  // extern "C"

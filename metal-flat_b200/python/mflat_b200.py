@@ -19,6 +19,7 @@ CUDA_LIB_PATH = os.path.join(LIB_DIR, "libmflat_cuda.so")
 
 METRICS = {"l2": 0, "ip": 1, "inner_product": 1, "cosine": 2}
 STORAGES = {"fp32": 0, "fp16": 1, "bf16": 2}
+SCORES = {"softmax": 0, "sigmoid": 1}
 STATUS = {0: "ok", 1: "null argument", 2: "bad argument", 3: "allocation failed",
           4: "index not built", 5: "internal error", 6: "device error", 7: "index file error"}
 
@@ -35,6 +36,9 @@ EXPORTS = [
     "mflat_coarse_create", "mflat_coarse_free", "mflat_coarse_train", "mflat_coarse_nlist",
     "mflat_coarse_size", "mflat_coarse_dim", "mflat_coarse_centroids", "mflat_coarse_csr",
     "mflat_coarse_probe", "mflat_coarse_set_shard",
+    "mflat_route_workspace_bytes", "mflat_route_device", "mflat_route_backward_device",
+    "mflat_beam_workspace_bytes", "mflat_beam_select_device", "mflat_beam_reorder_device",
+    "mflat_cache_workspace_bytes", "mflat_cache_evict_device",
 ]
 
 
@@ -48,6 +52,27 @@ class Timing(ctypes.Structure):
     _fields_ = [("total_ms", ctypes.c_float), ("screen_ms", ctypes.c_float),
                 ("select_ms", ctypes.c_float), ("screen_launches", ctypes.c_int),
                 ("launches", ctypes.c_int), ("fallback_queries", ctypes.c_int)]
+
+
+class RouterSpec(ctypes.Structure):
+    """mflat_router_t."""
+    _fields_ = [("experts", ctypes.c_int), ("k", ctypes.c_int), ("score", ctypes.c_int),
+                ("type", ctypes.c_int), ("renormalise", ctypes.c_int), ("groups", ctypes.c_int),
+                ("groups_kept", ctypes.c_int), ("group_top", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class BeamSpec(ctypes.Structure):
+    """mflat_beam_t."""
+    _fields_ = [("beams", ctypes.c_int), ("vocab", ctypes.c_int), ("k", ctypes.c_int),
+                ("type", ctypes.c_int), ("eos", ctypes.c_int)]
+
+
+class CacheSpec(ctypes.Structure):
+    """mflat_cache_t."""
+    _fields_ = [("heads", ctypes.c_int), ("group", ctypes.c_int), ("capacity", ctypes.c_int),
+                ("budget", ctypes.c_int), ("recent", ctypes.c_int), ("sink", ctypes.c_int),
+                ("type", ctypes.c_int), ("key_bytes", ctypes.c_int64), ("value_bytes", ctypes.c_int64),
+                ("key_stride", ctypes.c_int64 * 3), ("value_stride", ctypes.c_int64 * 3)]
 
 
 LOG_HANDLER = ctypes.CFUNCTYPE(None, ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
@@ -64,6 +89,7 @@ def lib() -> ctypes.CDLL:
         raise OSError(f"{LIB_PATH} is not built; run __graft_entry__.build() or make -C metal-flat_b200")
     L = ctypes.CDLL(LIB_PATH)
     vp, ci, cf = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    sz, i64 = ctypes.c_size_t, ctypes.c_int64
     i32p = ctypes.POINTER(ctypes.c_int32)
     f32p = ctypes.POINTER(ctypes.c_float)
     sig = {
@@ -106,6 +132,15 @@ def lib() -> ctypes.CDLL:
         "mflat_coarse_csr": ([vp, i32p, i32p], ci),
         "mflat_coarse_probe": ([vp, f32p, ci, ci, i32p], ci),
         "mflat_coarse_set_shard": ([vp, ci, ci, ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)], ci),
+        "mflat_route_workspace_bytes": ([vp, ci], sz),
+        "mflat_route_device": ([vp, vp, i64, ci] + [vp] * 7 + [sz, ci, vp], ci),
+        "mflat_route_backward_device": ([vp, vp, i64, ci, vp, vp, vp, i64, ci, vp], ci),
+        "mflat_beam_workspace_bytes": ([vp, ci], sz),
+        "mflat_beam_select_device": ([vp, vp, i64, vp, vp, ci, vp, vp, vp, vp, sz, ci, vp], ci),
+        "mflat_beam_reorder_device": ([vp, vp, i64, ci, ci, ci, ci, i64, i64, i64, i64, ci, vp], ci),
+        "mflat_cache_workspace_bytes": ([vp, ci], sz),
+        "mflat_cache_evict_device": ([vp, ci, vp, vp, vp, ci, ctypes.POINTER(i64)] + [vp] * 9
+                                     + [sz, ci, vp], ci),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -361,3 +396,119 @@ class CoarseQuantizer:
         _check(self._lib.mflat_coarse_probe(self._h, _ptr(q, ctypes.c_float), q.shape[0], int(nprobe),
                                             _ptr(out, ctypes.c_int32)), "coarse probe")
         return out
+
+
+def _code(table, v) -> int:
+    return table[v] if isinstance(v, str) else int(v)
+
+
+class Router:
+    """Routing to experts (mflat_route_device): scores, the k best experts of each
+    token, their weights, the lists by expert, and the gradient of the logits.
+
+    Pointers are device addresses (0 = none), as in FlatIndex.search_device; the
+    calls enqueue on `stream` and allocate nothing."""
+
+    def __init__(self, experts: int, k: int, score: str | int = "softmax", dtype: str | int = "fp32",
+                 renormalise: bool = False, scale: float = 1.0, groups: int = 1,
+                 groups_kept: int = 1, group_top: int = 1, device: int = -1):
+        self.spec = RouterSpec(int(experts), int(k), _code(SCORES, score), _code(STORAGES, dtype),
+                               int(bool(renormalise)), int(groups), int(groups_kept),
+                               int(group_top), float(scale))
+        self.device = int(device)
+        self._ref = ctypes.addressof(self.spec)
+        self._lib = lib()
+
+    def workspace_bytes(self, tokens: int) -> int:
+        return self._lib.mflat_route_workspace_bytes(self._ref, tokens)
+
+    def route_device(self, logits: int, tokens: int, ids: int, weights: int, stride: int = 0,
+                     bias: int = 0, mask: int = 0, start: int = 0, slots: int = 0, ws: int = 0,
+                     ws_bytes: int = 0, stream: int = 0) -> None:
+        """ids (int32) and weights (fp32), tokens x k; start (experts + 1) and slots
+        (tokens x k): entries t * k + j grouped by expert, as CoarseQuantizer.csr()
+        groups rows by cell."""
+        st = self._lib.mflat_route_device(self._ref, logits, stride, tokens, bias, mask, ids, weights,
+                                          start, slots, ws, ws_bytes, self.device, stream)
+        if st:
+            raise MflatError(st, "route")
+
+    def backward_device(self, logits: int, tokens: int, ids: int, grad_weights: int,
+                        grad_logits: int, stride: int = 0, grad_stride: int = 0,
+                        stream: int = 0) -> None:
+        """Gradient of the logits (their dtype) from the gradient of the weights."""
+        st = self._lib.mflat_route_backward_device(self._ref, logits, stride, tokens, ids,
+                                                   grad_weights, grad_logits, grad_stride,
+                                                   self.device, stream)
+        if st:
+            raise MflatError(st, "route backward")
+
+
+class BeamSearch:
+    """A beam search step over beams x vocabulary (mflat_beam_select_device)."""
+
+    def __init__(self, beams: int, vocab: int, k: int, dtype: str | int = "fp32", eos: int = -1,
+                 device: int = -1):
+        self.spec = BeamSpec(int(beams), int(vocab), int(k), _code(STORAGES, dtype), int(eos))
+        self.device = int(device)
+        self._ref = ctypes.addressof(self.spec)
+        self._lib = lib()
+
+    def workspace_bytes(self, batch: int) -> int:
+        return self._lib.mflat_beam_workspace_bytes(self._ref, batch)
+
+    def select_device(self, logits: int, cum: int, batch: int, parents: int, tokens: int,
+                      scores: int, stride: int = 0, finished: int = 0, ws: int = 0,
+                      ws_bytes: int = 0, stream: int = 0) -> None:
+        """parents, tokens (int32) and scores (fp32), batch x k, best first."""
+        st = self._lib.mflat_beam_select_device(self._ref, logits, stride, cum, finished, batch,
+                                                parents, tokens, scores, ws, ws_bytes, self.device,
+                                                stream)
+        if st:
+            raise MflatError(st, "beam select")
+
+
+def beam_reorder_device(states: int, parents: int, outer: int, batch: int, beams: int,
+                        segment_bytes: int, segments: int = 1, segment_stride: int = 0,
+                        row_stride: int = 0, outer_stride: int = 0, parent_stride: int = 0,
+                        device: int = -1, stream: int = 0) -> None:
+    """Rows of states follow their parent beams, in place (mflat_beam_reorder_device)."""
+    st = lib().mflat_beam_reorder_device(states, parents, parent_stride, outer, batch, beams,
+                                         segments, segment_bytes, segment_stride, row_stride,
+                                         outer_stride, device, stream)
+    if st:
+        raise MflatError(st, "beam reorder")
+
+
+class CacheEviction:
+    """Eviction from a key/value cache by accumulated attention weight
+    (mflat_cache_evict_device).  Strides are (sequence, head, slot) in bytes,
+    dense [sequence][head][slot][row] where not given."""
+
+    def __init__(self, heads: int, group: int, capacity: int, budget: int, key_bytes: int,
+                 value_bytes: int, recent: int = 0, sink: int = 0, dtype: str | int = "fp32",
+                 key_stride=(0, 0, 0), value_stride=(0, 0, 0), device: int = -1):
+        three = ctypes.c_int64 * 3
+        self.spec = CacheSpec(int(heads), int(group), int(capacity), int(budget), int(recent),
+                              int(sink), _code(STORAGES, dtype), int(key_bytes), int(value_bytes),
+                              three(*key_stride), three(*value_stride))
+        self.device = int(device)
+        self._ref = ctypes.addressof(self.spec)
+        self._lib = lib()
+
+    def workspace_bytes(self, batch: int) -> int:
+        return self._lib.mflat_cache_workspace_bytes(self._ref, batch)
+
+    def evict_device(self, batch: int, lens: int, seen: int, acc: int, pos: int, keys: int,
+                     values: int, out_lens: int, out_acc: int = 0, out_pos: int = 0,
+                     weights: int = 0, queries: int = 0, weight_stride=None, rows: int = 0,
+                     ws: int = 0, ws_bytes: int = 0, stream: int = 0) -> None:
+        """Adds the weights to acc and cuts every cache to the budget; out_acc and
+        out_pos default to acc and pos themselves."""
+        strides = None if weight_stride is None else (ctypes.c_int64 * 3)(*weight_stride)
+        st = self._lib.mflat_cache_evict_device(self._ref, batch, lens, seen, weights, queries,
+                                                strides, rows, acc, pos, out_acc or acc,
+                                                out_pos or pos, out_lens, keys, values, ws,
+                                                ws_bytes, self.device, stream)
+        if st:
+            raise MflatError(st, "cache evict")
