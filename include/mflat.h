@@ -304,7 +304,7 @@ MFLAT_API mflat_status_t mflat_route_backward_device(const mflat_router_t*, cons
  * lowest beam, then token.  A finished beam proposes only (eos, cum); logits of
  * -inf or NaN, and beams whose cum is not finite, propose nothing. */
 typedef struct {
-    int beams, vocab, k;            /* 1..MAX_BEAMS; >= 1; 1..MAX_K                 */
+    int beams, vocab, k;            /* 1..MAX_BEAMS; 1..2^30; 1..MAX_K              */
     mflat_storage_t type;           /* of the logits                                */
     int eos;                        /* token of finished beams, -1 = none finish    */
 } mflat_beam_t;

@@ -17,8 +17,10 @@
 namespace mflat_cu {
 namespace {
 
-constexpr int kMaxBeams = 64, kMaxBeamK = 128;
+constexpr int kMaxBeams = 64, kMaxBeamK = 128, kMaxVocab = 1 << 30;
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
+constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+constexpr int kListMax = 2048;      // candidates that a block filters into shared memory
 
 struct BeamParams {
     const void* logits;
@@ -26,112 +28,637 @@ struct BeamParams {
     const float* cum;
     const uint8_t* finished;
     int batch, beams, vocab, k, eos;
-    double* lse_sum;            // workspace, [rows]: sum of exp(x - max)
-    float* row_max;             // [rows]
-    float* cand_x;              // [rows][k]: best logits, best first (-inf: none)
-    int32_t* cand_v;            // [rows][k]: their tokens
+    int splits, per_split;      // segments of a row, and 16-byte packs in each
+    int rounds;                 // ceil(k / warps of a block)
+    uint64_t* cand;             // workspace, [rows][splits][k]: (logit key, ~token), best first, 0: none
+    double* part_sum;           // [rows][splits]: sum of exp(x - part_ref)
+    double* part_ref;
     int32_t* parents;
     int32_t* tokens;
     float* scores;
 };
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453094;
+// Logits beyond this leave the fast path: above it, or a segment with none above
+// kLow (the gap between the two is far below any sum's last digit).
+constexpr float kWild = 5e5f, kLow = -4e5f;
+
+__device__ __forceinline__ float exp2_fast(float t) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    return e;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 16 bytes of logits: as pairs of floats, and their maximum (which passes over NaN).
+template <class T>
+struct Logits {
+    static constexpr int N = 16 / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ float2 pair(int i) const {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
+        if constexpr (sizeof(T) == 4) {
+            return make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            return make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+        } else {
+            return __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        const float2 f = pair(i >> 1);
+        return (i & 1) ? f.y : f.x;
+    }
+    __device__ __forceinline__ float largest() const {
+        if constexpr (sizeof(T) == 4) {
+            const float2 a = pair(0), b = pair(1);
+            return fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
+        } else {
+            using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+            const T2* h = reinterpret_cast<const T2*>(&raw);
+            const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            return fmaxf(to_float(m.x), to_float(m.y));
+        }
+    }
+    __device__ __forceinline__ void fill(float v) {
+        T t[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = from_float<T>(v);
+        raw = *reinterpret_cast<const uint4*>(t);
+    }
+};
+
+// Bound of the relative error of a row's sum of exponentials, which is the
+// absolute error of its logarithm.  ex2 is off by 2^-22; t = x log2(e) - ref by half a
+// step of itself, 2^-24 |x - m| as a relative error of the term, and log2(e) in fp32 by
+// 2^-26 |x|; weighted by the term's share of the sum, |x - m| averages at most
+// ln(vocab).  A thread adds 8 or 4 terms at a time in fp32 (at most 7 steps of
+// 2^-24), all else is in 64 bits.
+__device__ __forceinline__ float sum_error(float m, int vocab) {
+    const float ln_v = __logf(static_cast<float>(vocab)) + 1.0f;
+    return 2.4e-7f + 4.5e-7f + 8e-8f * ln_v + 2e-8f * fabsf(m);
+}
+
+// a * 2^n for n <= 0.
+__device__ __forceinline__ double scale_down(double a, int n) {
+    return n < -1000 ? 0.0 : a * __longlong_as_double(static_cast<long long>(1023 + n) << 52);
+}
+
+// Ranks n entries by counting, for each, the better ones, eight threads an entry:
+// put(rank, i) is called for every entry that wanted(i) and whose rank is below most.
+template <class Wanted, class Better, class Put>
+__device__ __forceinline__ void rank_into(int n, int most, Wanted wanted, Better better, Put put) {
+    const int part = threadIdx.x & 7;
+    for (int i0 = 0; i0 < n; i0 += kRowThreads / 8) {
+        const int i = i0 + (threadIdx.x >> 3);
+        const bool want = i < n && wanted(i);
+        if (!__any_sync(kFullMask, want)) continue;
+        int rank = 0;
+        if (want)
+            for (int j = part; j < n; j += 8) rank += better(j, i) ? 1 : 0;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) rank += __shfl_xor_sync(kFullMask, rank, o);
+        if (want && part == 0 && rank < most) put(rank, i);
+    }
+}
+
+// The rounds-th largest of a warp's keys (one a lane); lane r < 4 also gets the
+// (r + 1)-th largest in `four` where there are as many rounds.
+template <class K>
+__device__ __forceinline__ K warp_floor(K mine, int rounds, K& four) {
+    K t = 0;
+    const int lane = threadIdx.x & 31;
+    for (int r = 0; r < rounds; ++r) {
+        if constexpr (sizeof(K) == 4) {
+            t = __reduce_max_sync(kFullMask, mine);
+        } else {
+            t = mine;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const K c = __shfl_xor_sync(kFullMask, t, o);
+                t = c > t ? c : t;
+            }
+        }
+        if (lane == r) four = t;
+        const unsigned who = __ballot_sync(kFullMask, mine == t);
+        if (lane == __ffs(who) - 1) mine = 0;
+    }
+    return t;
+}
+
+// Floor under the k best of what a block holds, from its threads' largest keys: at
+// least k of those reach it.  k <= 32: the k-th largest of the 8 warps' four largest
+// (a 32-lane bitonic sort in every warp; on random data about k entries reach it).
+// Above: the least of the warps' rounds-th largest.  One block barrier; calls in a
+// row pass sh of alternating halves.
+template <class K>
+struct FloorShared {
+    K top[kRowWarps][4];
+};
+template <class K>
+__device__ __forceinline__ K block_floor(K mine, int k, int rounds, FloorShared<K>& sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (k <= 32) {
+        K four = 0;
+        warp_floor(mine, 4, four);
+        if (lane < 4) sh.top[warp][lane] = four;
+        __syncthreads();
+        K v = sh.top[lane >> 2][lane & 3];
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+            for (int o = size >> 1; o > 0; o >>= 1) {
+                const K c = __shfl_xor_sync(kFullMask, v, o);
+                const bool larger = ((lane & size) == 0) == ((lane & o) == 0);
+                v = larger == (c > v) ? c : v;
+            }
+        return __shfl_sync(kFullMask, v, k - 1);
+    }
+    K unused = 0;
+    const K t = warp_floor(mine, rounds, unused);
+    if (lane == 0) sh.top[warp][0] = t;
+    __syncthreads();
+    K f = sh.top[0][0];
+#pragma unroll
+    for (int w = 1; w < kRowWarps; ++w) f = sh.top[w][0] < f ? sh.top[w][0] : f;
+    return f;
+}
+
 template <class V, class Op>
 __device__ V block_reduce(V v, Op op, V* sh) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kFullMask, v, o));
+    __syncthreads();
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
     __syncthreads();
     v = sh[0];
     for (int w = 1; w < kRowWarps; ++w) v = op(v, sh[w]);
-    __syncthreads();
     return v;
 }
 
+// The segment [t0, t1) of a row for any values: sum from 64-bit terms, the k best by
+// a radix select of the k-th key and an ordered pass for the lowest tokens among
+// its equals.  For NaN or infinities among the logits, sizes beyond kWild, and more
+// equals than the list holds.  `list` is scratch of at least k entries.
 template <class T>
-__global__ void __launch_bounds__(kRowThreads) beam_row_kernel(const BeamParams p) {
-    __shared__ uint64_t sh[kRowWarps];
-    const int64_t r = blockIdx.x;
-    const T* row = static_cast<const T*>(p.logits) + r * p.stride;
-    if (p.finished && p.finished[r]) return;
-    auto larger = [](auto a, auto b) { return a > b ? a : b; };
+__device__ __noinline__ void segment_exact(const BeamParams& p, const T* row, int t0, int t1,
+                                           int64_t part, uint64_t* list) {
+    __shared__ int hist[256];
+    __shared__ double sh_d[kRowWarps];
+    __shared__ int sh_count[kRowWarps];
+    __shared__ uint32_t sh_prefix;
+    __shared__ int sh_left, sh_n;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float m = neg_inf();
-    for (int v = threadIdx.x; v < p.vocab; v += kRowThreads) m = fmaxf(m, to_float(row[v]));
-    m = block_reduce(m, larger, reinterpret_cast<float*>(sh));
+    int valid = 0;
+    for (int v = t0 + threadIdx.x; v < t1; v += kRowThreads) {
+        const float x = to_float(row[v]);
+        m = fmaxf(m, x);
+        valid += x > neg_inf() ? 1 : 0;
+    }
+    m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, reinterpret_cast<float*>(sh_d));
+    valid = block_reduce(valid, [](int a, int b) { return a + b; }, sh_count);
     double sum = 0.0;
-    for (int v = threadIdx.x; v < p.vocab; v += kRowThreads) {
+    for (int v = t0 + threadIdx.x; v < t1; v += kRowThreads) {
         const float x = to_float(row[v]);
         if (x > neg_inf()) sum += x == m ? 1.0 : exp(static_cast<double>(x) - m);
     }
-    sum = block_reduce(sum, [](double a, double b) { return a + b; }, reinterpret_cast<double*>(sh));
+    sum = block_reduce(sum, [](double a, double b) { return a + b; }, sh_d);
+    const int want = min(p.k, valid);
+    uint64_t* out = p.cand + part * p.k;
+    for (int j = want + threadIdx.x; j < p.k; j += kRowThreads) out[j] = 0;
     if (threadIdx.x == 0) {
-        p.row_max[r] = m;
-        p.lse_sum[r] = sum;
+        p.part_ref[part] = m;
+        p.part_sum[part] = sum;
+        sh_prefix = 0;
+        sh_left = want;
+        sh_n = 0;
     }
-    // best first: (logit's key, then the lower token) as one number, each round
-    // the largest below the last
-    uint64_t last = ~0ull;
-    for (int j = 0; j < p.k; ++j) {
-        uint64_t best = 0;
-        for (int v = threadIdx.x; v < p.vocab; v += kRowThreads) {
-            const uint32_t key = choice_key(to_float(row[v]));
-            const uint64_t c = (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
-            if (key != 0u && c < last && c > best) best = c;
+    if (want == 0) return;
+    uint32_t mask = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = threadIdx.x; i < 256; i += kRowThreads) hist[i] = 0;
+        __syncthreads();
+        const uint32_t prefix = sh_prefix;
+        for (int v0 = t0; v0 < t1; v0 += kRowThreads) {
+            const int v = v0 + threadIdx.x;
+            const uint32_t key = v < t1 ? choice_key(to_float(row[v])) : 0u;
+            const bool in = key != 0u && (key & mask) == prefix;
+            const unsigned who = __ballot_sync(kFullMask, in);
+            if (!in) continue;
+            const unsigned d = (key >> shift) & 255u;
+            // a warp of one digit (ties) adds once
+            int same;
+            __match_all_sync(who, d, &same);
+            if (!same) atomicAdd(&hist[d], 1);
+            else if (lane == __ffs(who) - 1) atomicAdd(&hist[d], __popc(who));
         }
-        best = block_reduce(best, larger, sh);
-        last = best;
+        __syncthreads();
         if (threadIdx.x == 0) {
-            p.cand_x[r * p.k + j] = key_value(static_cast<uint32_t>(best >> 32));
-            p.cand_v[r * p.k + j] = best ? static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best)) : -1;
+            int left = sh_left, d = 255;
+            while (d > 0 && hist[d] < left) left -= hist[d--];
+            sh_prefix = prefix | (static_cast<uint32_t>(d) << shift);
+            sh_left = left;
         }
+        mask |= 255u << shift;
+        __syncthreads();
     }
+    const uint32_t cut = sh_prefix;
+    const int ties = sh_left;
+    int seen = 0;
+    for (int v0 = t0; v0 < t1; v0 += kRowThreads) {
+        const int v = v0 + threadIdx.x;
+        const uint32_t key = v < t1 ? choice_key(to_float(row[v])) : 0u;
+        const unsigned eq = __ballot_sync(kFullMask, key == cut);
+        __syncthreads();
+        if (lane == 0) sh_count[warp] = __popc(eq);
+        __syncthreads();
+        int rank = seen + __popc(eq & ((1u << lane) - 1u));
+        for (int w = 0; w < kRowWarps; ++w) {
+            rank += w < warp ? sh_count[w] : 0;
+            seen += sh_count[w];
+        }
+        if (key > cut || (key == cut && rank < ties))
+            list[atomicAdd(&sh_n, 1)] = (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
+    }
+    __syncthreads();
+    rank_into(want, want, [](int) { return true; }, [&](int j, int i) { return list[j] > list[i]; },
+              [&](int rank, int i) { out[rank] = list[i]; });
 }
 
-__global__ void __launch_bounds__(32) beam_merge_kernel(const BeamParams p) {
-    const int64_t b = blockIdx.x;
-    const int lane = threadIdx.x;
-    // lane l walks beams l and l + 32: its next candidate of each
-    int next[2] = {0, 0};
-    for (int j = 0; j < p.k; ++j) {
-        uint64_t best = 0;
-        int beam = INT_MAX, token = -1;
+// One segment of one row: its k best logits and its share of the sum.  The segment
+// is read once, PACKS loads of 16 bytes a thread in registers and the next ones on
+// their way.  The threads' largest logits so far give a floor under the k best
+// (block_floor), raised after chunks 1, 2, 4, 8, ...: only packs that reach it are
+// looked through, and what reaches it is listed, so later chunks list next to nothing.
+template <class T, int PACKS>
+__global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const BeamParams p) {
+    constexpr int N = Logits<T>::N, kChunk = PACKS * kRowThreads;
+    __shared__ uint64_t list[kListMax];
+    __shared__ FloorShared<uint32_t> sh_floor[2];
+    __shared__ double sh_sum[kRowWarps];
+    __shared__ int sh_ref[kRowWarps];
+    __shared__ uint32_t sh_top[kRowWarps];
+    __shared__ int sh_n, sh_odd;
+    const int64_t r = blockIdx.x / p.splits;
+    const int s = blockIdx.x % p.splits;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if ((p.finished && p.finished[r]) || !isfinite(p.cum[r])) return;
+    if (threadIdx.x == 0) { sh_n = 0; sh_odd = 0; }
+    const T* row = static_cast<const T*>(p.logits) + r * p.stride;
+    // packs are counted from the 16-byte boundary at or below the row's start
+    const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int start = s * p.per_split * N - skew;
+    const int t0 = start + static_cast<int>(threadIdx.x) * N;
+    auto token_of = [&](int c, int q) { return t0 + (c * PACKS + q) * (kRowThreads * N); };
+    auto load = [&](int c, Logits<T> (&v)[PACKS]) {
+        if ((c + 1) * kChunk <= p.per_split && start + c * kChunk * N >= 0 &&
+            start + (c + 1) * kChunk * N <= p.vocab) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int w = lane + 32 * h;
-            if (w >= p.beams || next[h] >= p.k) continue;
-            const int64_t r = b * p.beams + w;
-            const float cum = p.cum[r];
-            if (!isfinite(cum)) continue;
-            const bool done = p.finished && p.finished[r];
-            double key;
-            int v;
-            if (done) {
-                if (next[h] > 0) continue;
-                key = cum;
-                v = p.eos;
+            for (int q = 0; q < PACKS; ++q)
+                v[q].raw = *reinterpret_cast<const uint4*>(row + token_of(c, q));
+            return;
+        }
+#pragma unroll
+        for (int q = 0; q < PACKS; ++q) {
+            const int e = token_of(c, q);
+            if ((c * PACKS + q) * kRowThreads + static_cast<int>(threadIdx.x) >= p.per_split || e >= p.vocab) {
+                v[q].fill(neg_inf());
+            } else if (e >= 0 && e + N <= p.vocab) {
+                v[q].raw = *reinterpret_cast<const uint4*>(row + e);
             } else {
-                const float x = p.cand_x[r * p.k + next[h]];
-                if (!(x > neg_inf())) continue;
-                const float m = p.row_max[r];
-                key = cum + ((x == m ? 0.0 : static_cast<double>(x) - m) - log(p.lse_sum[r]));
-                v = p.cand_v[r * p.k + next[h]];
-            }
-            const uint64_t c = choice_key(key);
-            if (c > best) { best = c; beam = w; token = v; }
-        }
-        uint64_t top = best;
+                T t[N];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint64_t c = __shfl_xor_sync(kFullMask, top, o);
-            top = c > top ? c : top;
+                for (int i = 0; i < N; ++i)
+                    t[i] = e + i >= 0 && e + i < p.vocab ? row[e + i] : from_float<T>(neg_inf());
+                v[q].raw = *reinterpret_cast<const uint4*>(t);
+            }
         }
-        const int who = __reduce_min_sync(kFullMask, best == top ? beam : INT_MAX);
-        token = __shfl_sync(kFullMask, token, who & 31);
-        if (top != 0 && (who & 31) == lane) ++next[who >> 5];
+    };
+    const int chunks = (p.per_split + kChunk - 1) / kChunk;
+    Logits<T> next[PACKS];
+    load(0, next);
+    float best = neg_inf(), floor_x = 0.0f;
+    uint32_t floor_b = 0;
+    double sum = 0.0;
+    float ref = 0.0f;           // a whole number: sums of other references scale by powers of 2
+    bool any = false, odd = false;
+    int turn = 0;
+    for (int c = 0; c < chunks; ++c) {
+        Logits<T> v[PACKS];
+#pragma unroll
+        for (int q = 0; q < PACKS; ++q) v[q] = next[q];
+        if (c + 1 < chunks) load(c + 1, next);
+        else grid_release();
+        float most[PACKS], m = neg_inf();
+#pragma unroll
+        for (int q = 0; q < PACKS; ++q) {
+            most[q] = v[q].largest();
+            m = fmaxf(m, most[q]);
+        }
+        best = fmaxf(best, m);
+        odd |= m > kWild;
+        if (m >= -kWild && m <= kWild) {
+            const float mine = m * kLog2e;
+            if (!any || mine > ref + 60.0f) {
+                const float now = rintf(mine);
+                sum = any ? scale_down(sum, static_cast<int>(ref - now)) : 0.0;
+                ref = now;
+                any = true;
+            }
+            const float2 l2 = make_float2(kLog2e, kLog2e), shift = make_float2(-ref, -ref);
+            double chunk = 0.0;
+#pragma unroll
+            for (int q = 0; q < PACKS; ++q) {
+                float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    const float2 t = fma2(v[q].pair(i), l2, shift);
+                    part = add2(part, make_float2(exp2_fast(t.x), exp2_fast(t.y)));
+                }
+                chunk += static_cast<double>(part.x + part.y);
+            }
+            sum += chunk;
+            odd |= chunk != chunk;      // NaN among the logits
+        }
+        if ((c & (c + 1)) == 0 || c + 1 == chunks) {
+            floor_b = block_floor(choice_key(best), p.k, p.rounds, sh_floor[turn & 1]);
+            ++turn;
+            // everything above -inf where fewer than k were seen
+            floor_x = floor_b == 0u ? -3.402823466e38f : key_value(floor_b);
+        }
+#pragma unroll
+        for (int q = 0; q < PACKS; ++q) {
+            if (!(most[q] >= floor_x)) continue;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float x = v[q].at(i);
+                if (x >= floor_x) {
+                    const int at = atomicAdd(&sh_n, 1);
+                    if (at < kListMax)
+                        list[at] = (static_cast<uint64_t>(choice_key(x)) << 32) |
+                                   (0xffffffffu - static_cast<uint32_t>(token_of(c, q) + i));
+                }
+            }
+        }
+    }
+    // the block's largest logit and sum
+    const uint32_t top_w = __reduce_max_sync(kFullMask, choice_key(best));
+    const int ref_w = __reduce_max_sync(kFullMask, any ? static_cast<int>(ref) : INT_MIN / 2);
+    if (any) sum = scale_down(sum, static_cast<int>(ref) - ref_w);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+    if (lane == 0) {
+        sh_top[warp] = top_w;
+        sh_sum[warp] = sum;
+        sh_ref[warp] = ref_w;
+    }
+    if (odd) sh_odd = 1;
+    __syncthreads();
+    uint32_t top = sh_top[0];
+    int ref_b = sh_ref[0];
+#pragma unroll
+    for (int w = 1; w < kRowWarps; ++w) {
+        top = max(top, sh_top[w]);
+        ref_b = max(ref_b, sh_ref[w]);
+    }
+    const int n = sh_n;
+    if (sh_odd || n > kListMax || (top != 0u && key_value(top) < kLow)) {
+        const int from = max(start, 0);
+        const int to = static_cast<int>(min(static_cast<int64_t>(start) + static_cast<int64_t>(p.per_split) * N,
+                                            static_cast<int64_t>(p.vocab)));
+        segment_exact(p, row, from, to, blockIdx.x, list);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        double total = 0.0;
+        for (int w = 0; w < kRowWarps; ++w) total += scale_down(sh_sum[w], sh_ref[w] - ref_b);
+        p.part_ref[blockIdx.x] = top == 0u ? static_cast<double>(neg_inf()) : ref_b * kLn2;
+        p.part_sum[blockIdx.x] = total;
+    }
+    uint64_t* out = p.cand + static_cast<int64_t>(blockIdx.x) * p.k;
+    const uint64_t least = static_cast<uint64_t>(floor_b) << 32;
+    rank_into(n, p.k, [&](int i) { return list[i] >= least; },
+              [&](int j, int i) { return list[j] > list[i]; }, [&](int rank, int i) { out[rank] = list[i]; });
+    for (int j = n + threadIdx.x; j < p.k; j += kRowThreads) out[j] = 0;
+}
+
+struct Choice {
+    uint64_t key;       // choice_key of cum + log p in 64 bits
+    uint64_t at;        // beam, token
+};
+__device__ __forceinline__ bool better(const Choice& a, const Choice& b) {
+    return a.key > b.key || (a.key == b.key && a.at < b.at);
+}
+
+// One sequence: its beams' sums, then the k best of the chunks' candidates.
+template <class T>
+__global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParams p) {
+    __shared__ double sh_base[kMaxBeams];       // cum - log sum exp(x - ref); NaN: no candidates
+    __shared__ double sh_ref[kMaxBeams];
+    __shared__ float sh_off[kMaxBeams];         // error of that
+    __shared__ int sh_redo[kMaxBeams];
+    __shared__ Choice list[kListMax];
+    __shared__ Choice best[kMaxBeamK];
+    __shared__ FloorShared<uint64_t> sh_floor;
+    __shared__ double sh_sum[kRowWarps];
+    __shared__ float sh_err;
+    __shared__ int sh_n, sh_again;
+    const int64_t b = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    grid_wait();
+    for (int w = warp; w < p.beams; w += kRowWarps) {
+        const int64_t r = b * p.beams + w;
+        const float cum = p.cum[r];
+        const bool done = p.finished && p.finished[r];
+        double base = __longlong_as_double(0x7ff8000000000000ll), sum = 0.0;
+        const double none = static_cast<double>(neg_inf());
+        double ref = none;
+        if (isfinite(cum) && !done) {
+            for (int s = lane; s < p.splits; s += 32) ref = fmax(ref, p.part_ref[r * p.splits + s]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ref = fmax(ref, __shfl_xor_sync(kFullMask, ref, o));
+            for (int s = lane; s < p.splits; s += 32) {
+                const double f = p.part_ref[r * p.splits + s];
+                if (f > none) {
+                    const double part = p.part_sum[r * p.splits + s];
+                    sum += f == ref ? part : part * exp(f - ref);
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+            if (ref > none) base = static_cast<double>(cum) - log(sum);
+        } else if (isfinite(cum)) {
+            base = cum;
+        }
         if (lane == 0) {
-            p.parents[b * p.k + j] = top ? who : -1;
-            p.tokens[b * p.k + j] = top ? token : -1;
-            p.scores[b * p.k + j] = static_cast<float>(key_value(top));
+            sh_base[w] = base;
+            sh_ref[w] = ref;
+            // exact beyond kWild (segment_exact's sums)
+            const bool fast = ref > -2.0 * kWild && ref < 2.0 * kWild;
+            sh_off[w] = fast ? sum_error(static_cast<float>(ref), p.vocab) : 0.0f;
+            sh_redo[w] = 0;
         }
+    }
+    const int per_beam = p.splits * p.k, total = p.beams * per_beam;
+    const uint64_t* cand = p.cand + b * total;
+    auto choice_of = [&](int i) {
+        Choice c{0, 0};
+        const int w = i / per_beam;
+        const double base = sh_base[w];
+        if (base != base) return c;
+        c.at = static_cast<uint64_t>(w) << 32;
+        if (p.finished && p.finished[b * p.beams + w]) {
+            if (i == w * per_beam) {
+                c.key = choice_key(base);
+                c.at |= static_cast<uint32_t>(p.eos);
+            }
+            return c;
+        }
+        const uint64_t v = cand[i];
+        const uint32_t key = static_cast<uint32_t>(v >> 32);
+        if (key == 0u) return c;
+        const float x = key_value(key);
+        c.at |= 0xffffffffu - static_cast<uint32_t>(v);
+        // +inf: only it counts, key = cum - log(how many)
+        if (sh_ref[w] < static_cast<double>(-neg_inf())) c.key = choice_key(base + (static_cast<double>(x) - sh_ref[w]));
+        else if (x == -neg_inf()) c.key = choice_key(base);
+        return c;
+    };
+    for (int attempt = 0; ; ++attempt) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sh_n = 0;
+            sh_again = 0;
+            float e = 0.0f;
+            for (int w = 0; w < p.beams; ++w) e = fmaxf(e, sh_off[w]);
+            sh_err = 2.0f * e;
+        }
+        uint64_t mine = 0;
+        for (int i = threadIdx.x; i < total; i += kRowThreads) {
+            const uint64_t key = choice_of(i).key;
+            mine = key > mine ? key : mine;
+        }
+        uint64_t floor_b = block_floor(mine, p.k, p.rounds, sh_floor);
+        // a key below the floor by less than the sums' error could belong above it
+        if (floor_b != 0) floor_b = choice_key(key_value(floor_b) - static_cast<double>(sh_err));
+        if (floor_b == 0) floor_b = 1;
+        if (mine >= floor_b) {
+            for (int i = threadIdx.x; i < total; i += kRowThreads) {
+                const Choice c = choice_of(i);
+                if (c.key < floor_b) continue;
+                const int at = atomicAdd(&sh_n, 1);
+                if (at < kListMax) list[at] = c;
+            }
+        }
+        for (int j = threadIdx.x; j < p.k; j += kRowThreads) best[j] = Choice{0, 0};
+        __syncthreads();
+        const int n = min(sh_n, kListMax);
+        if (sh_n <= kListMax) {
+            rank_into(n, p.k, [](int) { return true; },
+                      [&](int j, int i) { return better(list[j], list[i]); },
+                      [&](int rank, int i) { best[rank] = list[i]; });
+            __syncthreads();
+        } else {
+            // more equal keys than the list holds: one block-wide best per place
+            Choice last{~0ull, 0};
+            for (int j = 0; j < p.k; ++j) {
+                Choice c{0, 0};
+                for (int i = threadIdx.x; i < total; i += kRowThreads) {
+                    const Choice x = choice_of(i);
+                    if (x.key != 0 && better(last, x) && better(x, c)) c = x;
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    Choice x;
+                    x.key = __shfl_xor_sync(kFullMask, c.key, o);
+                    x.at = __shfl_xor_sync(kFullMask, c.at, o);
+                    if (better(x, c)) c = x;
+                }
+                __syncthreads();
+                if (lane == 0) list[warp] = c;
+                __syncthreads();
+                c = list[0];
+                for (int w = 1; w < kRowWarps; ++w)
+                    if (better(list[w], c)) c = list[w];
+                last = c;
+                if (threadIdx.x == 0) best[j] = c;
+                if (c.key == 0) break;
+            }
+            __syncthreads();
+        }
+        if (attempt == 2) break;
+        // Two beams' candidates closer than their sums' errors, in the selection or
+        // across its end: those beams' sums are formed again from 64-bit terms.
+        const Choice last = best[p.k - 1];
+        auto close = [&](const Choice& x, const Choice& y) {
+            const int u = static_cast<int>(x.at >> 32), w = static_cast<int>(y.at >> 32);
+            if (x.key == 0 || y.key == 0 || u == w) return;
+            const double off = static_cast<double>(sh_off[u]) + sh_off[w];
+            if (off > 0.0 && !(key_value(x.key) - key_value(y.key) > off)) {
+                sh_redo[u] = sh_redo[w] = 1;
+                sh_again = 1;
+            }
+        };
+        for (int j = threadIdx.x; j + 1 < p.k; j += kRowThreads) close(best[j], best[j + 1]);
+        if (sh_n <= kListMax) {
+            for (int i = threadIdx.x; i < n; i += kRowThreads)
+                if (better(last, list[i])) close(last, list[i]);
+        } else {
+            for (int i = threadIdx.x; i < total; i += kRowThreads) {
+                const Choice c = choice_of(i);
+                if (better(last, c)) close(last, c);
+            }
+        }
+        __syncthreads();
+        if (!sh_again) break;
+        for (int w = 0; w < p.beams; ++w) {
+            if (attempt == 0 && !sh_redo[w]) continue;
+            if (sh_off[w] == 0.0f) continue;
+            const int64_t r = b * p.beams + w;
+            const T* row = static_cast<const T*>(p.logits) + r * p.stride;
+            const double m = sh_ref[w];
+            double sum = 0.0;
+            for (int v = threadIdx.x; v < p.vocab; v += kRowThreads) {
+                const float x = to_float(row[v]);
+                if (x > neg_inf()) sum += exp(static_cast<double>(x) - m);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+            __syncthreads();
+            if (lane == 0) sh_sum[warp] = sum;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                double all = 0.0;
+                for (int i = 0; i < kRowWarps; ++i) all += sh_sum[i];
+                sh_base[w] = static_cast<double>(p.cum[r]) - log(all);
+                sh_off[w] = 0.0f;
+            }
+        }
+    }
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) {
+        const Choice c = best[j];
+        p.parents[b * p.k + j] = c.key ? static_cast<int32_t>(c.at >> 32) : -1;
+        p.tokens[b * p.k + j] = c.key ? static_cast<int32_t>(c.at & 0xffffffffu) : -1;
+        p.scores[b * p.k + j] = static_cast<float>(key_value(c.key));
     }
 }
 
@@ -192,20 +719,42 @@ cudaError_t launch_reorder(const ReorderParams& p, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
-
-struct BeamLayout {
-    size_t sum, max, x, v, end;
+// How rows are cut.  A block holds 4 packs of 16 bytes a thread at a time (16 KB) and
+// runs through its segment.  Where all segments of one chunk would not fill the
+// machine twice, chunks shrink to 2 or 1 packs a thread, for more blocks.  Else
+// the segments are as long as leaves the fewest chunks in a row on a slot (4 blocks an
+// SM), each segment counting 1.5 more for its floor, list and results.
+struct BeamPlan {
+    int packs, splits, per_split;
+    size_t cand, sum, ref, end;
 };
-BeamLayout beam_layout(const mflat_cu_beam_t* b, int batch) {
-    const size_t rows = static_cast<size_t>(batch) * b->beams;
-    BeamLayout l;
-    l.sum = 0;
-    l.max = l.sum + round256(rows * 8);
-    l.x = l.max + round256(rows * 4);
-    l.v = l.x + round256(rows * b->k * 4);
-    l.end = l.v + round256(rows * b->k * 4);
-    return l;
+BeamPlan beam_plan(const mflat_cu_beam_t* b, int batch) {
+    const int n = static_cast<int>(16 / type_bytes(b->type));
+    const int64_t rows = static_cast<int64_t>(batch) * b->beams;
+    // a row may start anywhere in its first pack
+    const int64_t row_packs = (static_cast<int64_t>(b->vocab) + 2 * (n - 1)) / n;
+    auto chunks_of = [&](int packs) { return (row_packs + packs * kRowThreads - 1) / (packs * kRowThreads); };
+    BeamPlan p{};
+    p.packs = 4;
+    while (p.packs > 1 && rows * chunks_of(p.packs) < 2 * 148) p.packs /= 2;
+    const int64_t chunks = chunks_of(p.packs), slots = 4 * 148;
+    double least = 1e300;
+    for (int64_t s = 1; s <= chunks; ++s) {
+        const double cost = static_cast<double>((rows * s + slots - 1) / slots) *
+                            (static_cast<double>((chunks + s - 1) / s) + 1.5);
+        if (cost < least) {
+            least = cost;
+            p.splits = static_cast<int>(s);
+        }
+        if (s >= 256) break;
+    }
+    p.per_split = static_cast<int>((row_packs + p.splits - 1) / p.splits);
+    const size_t parts = static_cast<size_t>(rows) * p.splits;
+    p.cand = 0;
+    p.sum = p.cand + round256(parts * b->k * 8);
+    p.ref = p.sum + round256(parts * 8);
+    p.end = p.ref + round256(parts * 8);
+    return p;
 }
 
 int check_beam(const mflat_cu_beam_t* b, int batch) {
@@ -218,7 +767,10 @@ int check_beam(const mflat_cu_beam_t* b, int batch) {
         std::snprintf(msg, sizeof msg, "k=%d outside [1, %d]", b->k, kMaxBeamK);
         return fail(ST_BAD_ARG, msg);
     }
-    if (b->vocab < 1) return fail(ST_BAD_ARG, "vocab below 1");
+    if (b->vocab < 1 || b->vocab > kMaxVocab) {
+        std::snprintf(msg, sizeof msg, "vocab=%d outside [1, %d]", b->vocab, kMaxVocab);
+        return fail(ST_BAD_ARG, msg);
+    }
     if (b->type < 0 || b->type > 2) return fail(ST_BAD_ARG, "unknown logits type");
     if (b->eos < -1 || b->eos >= b->vocab) return fail(ST_BAD_ARG, "eos outside [-1, vocab)");
     if (batch < 0 || static_cast<int64_t>(batch) * b->beams * b->k > INT_MAX) {
@@ -235,7 +787,7 @@ using namespace mflat_cu;
 
 extern "C" size_t mflat_cu_beam_workspace(const mflat_cu_beam_t* b, int batch) {
     if (check_beam(b, batch) != ST_OK) return 0;
-    return beam_layout(b, batch).end;
+    return beam_plan(b, batch).end;
 }
 
 extern "C" int mflat_cu_beam_select(const mflat_cu_beam_t* b, const void* logits, int64_t stride,
@@ -251,7 +803,9 @@ extern "C" int mflat_cu_beam_select(const mflat_cu_beam_t* b, const void* logits
         !aligned_to(tokens, 4) || !aligned_to(scores, 4))
         return fail(ST_BAD_ARG, "misaligned pointer");
     if (batch == 0) return ST_OK;
-    const BeamLayout l = beam_layout(b, batch);
+    const BeamPlan l = beam_plan(b, batch);
+    if (static_cast<int64_t>(batch) * b->beams * l.splits > INT_MAX)
+        return fail(ST_BAD_ARG, "batch * beams * vocab too large for one call");
     if (!ws || ws_bytes < l.end || !aligned_to(ws, 256))
         return fail(ST_BAD_ARG, "workspace missing, too small or not 256-byte aligned");
     rc = operator_device(device, &device);
@@ -269,19 +823,27 @@ extern "C" int mflat_cu_beam_select(const mflat_cu_beam_t* b, const void* logits
     p.vocab = b->vocab;
     p.k = b->k;
     p.eos = b->eos;
-    p.lse_sum = reinterpret_cast<double*>(w + l.sum);
-    p.row_max = reinterpret_cast<float*>(w + l.max);
-    p.cand_x = reinterpret_cast<float*>(w + l.x);
-    p.cand_v = reinterpret_cast<int32_t*>(w + l.v);
+    p.splits = l.splits;
+    p.per_split = l.per_split;
+    p.rounds = (b->k + kRowWarps - 1) / kRowWarps;
+    p.cand = reinterpret_cast<uint64_t*>(w + l.cand);
+    p.part_sum = reinterpret_cast<double*>(w + l.sum);
+    p.part_ref = reinterpret_cast<double*>(w + l.ref);
     p.parents = parents;
     p.tokens = tokens;
     p.scores = scores;
     CU_TRY(with_type(b->type, [&](auto zero) {
-        beam_row_kernel<decltype(zero)><<<batch * b->beams, kRowThreads, 0, st>>>(p);
-        return cudaGetLastError();
-    }), "beam rows launch");
-    beam_merge_kernel<<<batch, 32, 0, st>>>(p);
-    CU_TRY(cudaGetLastError(), "beam merge launch");
+        using T = decltype(zero);
+        const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(batch) * b->beams * l.splits);
+        switch (l.packs) {
+            case 1: beam_segment_kernel<T, 1><<<grid, kRowThreads, 0, st>>>(p); break;
+            case 2: beam_segment_kernel<T, 2><<<grid, kRowThreads, 0, st>>>(p); break;
+            default: beam_segment_kernel<T, 4><<<grid, kRowThreads, 0, st>>>(p); break;
+        }
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        return launch_after(beam_merge_kernel<T>, dim3(batch), kRowThreads, 0, st, p);
+    }), "beam select launch");
     return ST_OK;
 }
 
