@@ -20,7 +20,9 @@ namespace {
 constexpr int kMaxBeams = 64, kMaxBeamK = 128, kMaxVocab = 1 << 30;
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
-constexpr int kListMax = 2048;      // candidates that a block filters into shared memory
+constexpr int kListMax = 1024;      // candidates that a block filters into shared memory
+constexpr int kHeld = 4;            // candidates a thread of the merge holds
+constexpr int kPackMax = 512;       // 16-byte packs set aside on the way
 
 struct BeamParams {
     const void* logits;
@@ -106,15 +108,26 @@ struct Logits {
     }
 };
 
+// One add per thread, as written (few threads come here at a time, so gathering a
+// warp's adds first costs more than it saves).
+__device__ __forceinline__ int shared_add(int* p, int v) {
+    int old;
+    asm volatile("atom.shared.add.s32 %0, [%1], %2;"
+                 : "=r"(old)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(v)
+                 : "memory");
+    return old;
+}
+
 // Bound of the relative error of a row's sum of exponentials, which is the
 // absolute error of its logarithm.  ex2 is off by 2^-22; t = x log2(e) - ref by half a
 // step of itself, 2^-24 |x - m| as a relative error of the term, and log2(e) in fp32 by
 // 2^-26 |x|; weighted by the term's share of the sum, |x - m| averages at most
-// ln(vocab).  A thread adds 8 or 4 terms at a time in fp32 (at most 7 steps of
-// 2^-24), all else is in 64 bits.
+// ln(vocab).  A thread adds at most 64 terms in fp32, up to 4 in a row by twos and
+// then 8 such parts (13 steps of 2^-24), all else is in 64 bits.
 __device__ __forceinline__ float sum_error(float m, int vocab) {
     const float ln_v = __logf(static_cast<float>(vocab)) + 1.0f;
-    return 2.4e-7f + 4.5e-7f + 8e-8f * ln_v + 2e-8f * fabsf(m);
+    return 2.4e-7f + 7.8e-7f + 8e-8f * ln_v + 2e-8f * fabsf(m);
 }
 
 // a * 2^n for n <= 0.
@@ -123,13 +136,13 @@ __device__ __forceinline__ double scale_down(double a, int n) {
 }
 
 // Ranks n entries by counting, for each, the better ones, eight threads an entry:
-// put(rank, i) is called for every entry that wanted(i) and whose rank is below most.
-template <class Wanted, class Better, class Put>
-__device__ __forceinline__ void rank_into(int n, int most, Wanted wanted, Better better, Put put) {
+// put(rank, i) is called for every entry whose rank is below most.
+template <class Better, class Put>
+__device__ __forceinline__ void rank_into(int n, int most, Better better, Put put) {
     const int part = threadIdx.x & 7;
     for (int i0 = 0; i0 < n; i0 += kRowThreads / 8) {
         const int i = i0 + (threadIdx.x >> 3);
-        const bool want = i < n && wanted(i);
+        const bool want = i < n;
         if (!__any_sync(kFullMask, want)) continue;
         int rank = 0;
         if (want)
@@ -142,21 +155,11 @@ __device__ __forceinline__ void rank_into(int n, int most, Wanted wanted, Better
 
 // The rounds-th largest of a warp's keys (one a lane); lane r < 4 also gets the
 // (r + 1)-th largest in `four` where there are as many rounds.
-template <class K>
-__device__ __forceinline__ K warp_floor(K mine, int rounds, K& four) {
-    K t = 0;
+__device__ __forceinline__ uint32_t warp_floor(uint32_t mine, int rounds, uint32_t& four) {
+    uint32_t t = 0;
     const int lane = threadIdx.x & 31;
     for (int r = 0; r < rounds; ++r) {
-        if constexpr (sizeof(K) == 4) {
-            t = __reduce_max_sync(kFullMask, mine);
-        } else {
-            t = mine;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const K c = __shfl_xor_sync(kFullMask, t, o);
-                t = c > t ? c : t;
-            }
-        }
+        t = __reduce_max_sync(kFullMask, mine);
         if (lane == r) four = t;
         const unsigned who = __ballot_sync(kFullMask, mine == t);
         if (lane == __ffs(who) - 1) mine = 0;
@@ -169,34 +172,33 @@ __device__ __forceinline__ K warp_floor(K mine, int rounds, K& four) {
 // (a 32-lane bitonic sort in every warp; on random data about k entries reach it).
 // Above: the least of the warps' rounds-th largest.  One block barrier; calls in a
 // row pass sh of alternating halves.
-template <class K>
 struct FloorShared {
-    K top[kRowWarps][4];
+    uint32_t top[kRowWarps][4];
 };
-template <class K>
-__device__ __forceinline__ K block_floor(K mine, int k, int rounds, FloorShared<K>& sh) {
+__device__ __forceinline__ uint32_t block_floor(uint32_t mine, int k, int rounds, FloorShared& sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (k <= 32) {
-        K four = 0;
+        uint32_t four = 0;
         warp_floor(mine, 4, four);
-        if (lane < 4) sh.top[warp][lane] = four;
+        // the fours come sorted: every other one backwards is the sort's third step
+        if (lane < 4) sh.top[warp][(warp & 1) ? 3 - lane : lane] = four;
         __syncthreads();
-        K v = sh.top[lane >> 2][lane & 3];
+        uint32_t v = sh.top[lane >> 2][lane & 3];
 #pragma unroll
-        for (int size = 2; size <= 32; size <<= 1)
+        for (int size = 8; size <= 32; size <<= 1)
 #pragma unroll
             for (int o = size >> 1; o > 0; o >>= 1) {
-                const K c = __shfl_xor_sync(kFullMask, v, o);
+                const uint32_t c = __shfl_xor_sync(kFullMask, v, o);
                 const bool larger = ((lane & size) == 0) == ((lane & o) == 0);
                 v = larger == (c > v) ? c : v;
             }
         return __shfl_sync(kFullMask, v, k - 1);
     }
-    K unused = 0;
-    const K t = warp_floor(mine, rounds, unused);
+    uint32_t unused = 0;
+    const uint32_t t = warp_floor(mine, rounds, unused);
     if (lane == 0) sh.top[warp][0] = t;
     __syncthreads();
-    K f = sh.top[0][0];
+    uint32_t f = sh.top[0][0];
 #pragma unroll
     for (int w = 1; w < kRowWarps; ++w) f = sh.top[w][0] < f ? sh.top[w][0] : f;
     return f;
@@ -214,13 +216,14 @@ __device__ V block_reduce(V v, Op op, V* sh) {
     return v;
 }
 
-// The segment [t0, t1) of a row for any values: sum from 64-bit terms, the k best by
-// a radix select of the k-th key and an ordered pass for the lowest tokens among
-// its equals.  For NaN or infinities among the logits, sizes beyond kWild, and more
-// equals than the list holds.  `list` is scratch of at least k entries.
+// The segment [t0, t1) of a row for any values: the k best by a radix select of the
+// k-th key and an ordered pass for the lowest tokens among its equals, and with
+// `sums` the sum from 64-bit terms.  For NaN or infinities among the logits and sizes
+// beyond kWild (with sums), and for more equals than the lists hold.  `list` is scratch
+// of at least k entries.
 template <class T>
 __device__ __noinline__ void segment_exact(const BeamParams& p, const T* row, int t0, int t1,
-                                           int64_t part, uint64_t* list) {
+                                           int64_t part, bool sums, uint64_t* list) {
     __shared__ int hist[256];
     __shared__ double sh_d[kRowWarps];
     __shared__ int sh_count[kRowWarps];
@@ -236,18 +239,22 @@ __device__ __noinline__ void segment_exact(const BeamParams& p, const T* row, in
     }
     m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, reinterpret_cast<float*>(sh_d));
     valid = block_reduce(valid, [](int a, int b) { return a + b; }, sh_count);
-    double sum = 0.0;
-    for (int v = t0 + threadIdx.x; v < t1; v += kRowThreads) {
-        const float x = to_float(row[v]);
-        if (x > neg_inf()) sum += x == m ? 1.0 : exp(static_cast<double>(x) - m);
+    if (sums) {
+        double sum = 0.0;
+        for (int v = t0 + threadIdx.x; v < t1; v += kRowThreads) {
+            const float x = to_float(row[v]);
+            if (x > neg_inf()) sum += x == m ? 1.0 : exp(static_cast<double>(x) - m);
+        }
+        sum = block_reduce(sum, [](double a, double b) { return a + b; }, sh_d);
+        if (threadIdx.x == 0) {
+            p.part_ref[part] = m;
+            p.part_sum[part] = sum;
+        }
     }
-    sum = block_reduce(sum, [](double a, double b) { return a + b; }, sh_d);
     const int want = min(p.k, valid);
     uint64_t* out = p.cand + part * p.k;
     for (int j = want + threadIdx.x; j < p.k; j += kRowThreads) out[j] = 0;
     if (threadIdx.x == 0) {
-        p.part_ref[part] = m;
-        p.part_sum[part] = sum;
         sh_prefix = 0;
         sh_left = want;
         sh_n = 0;
@@ -297,32 +304,34 @@ __device__ __noinline__ void segment_exact(const BeamParams& p, const T* row, in
             seen += sh_count[w];
         }
         if (key > cut || (key == cut && rank < ties))
-            list[atomicAdd(&sh_n, 1)] = (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
+            list[shared_add(&sh_n, 1)] = (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
     }
     __syncthreads();
-    rank_into(want, want, [](int) { return true; }, [&](int j, int i) { return list[j] > list[i]; },
+    rank_into(want, want, [&](int j, int i) { return list[j] > list[i]; },
               [&](int rank, int i) { out[rank] = list[i]; });
 }
 
 // One segment of one row: its k best logits and its share of the sum.  The segment
-// is read once, PACKS loads of 16 bytes a thread in registers and the next ones on
-// their way.  The threads' largest logits so far give a floor under the k best
-// (block_floor), raised after chunks 1, 2, 4, 8, ...: only packs that reach it are
-// looked through, and what reaches it is listed, so later chunks list next to nothing.
+// is read once, PACKS packs of 16 bytes a thread at a time.  The threads' largest
+// logits so far give a floor under the k best (block_floor), raised after chunks 1, 4
+// and the last: only packs that reach it are set aside, few in later chunks, and looked
+// through at the end.
 template <class T, int PACKS>
-__global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const __grid_constant__ BeamParams p) {
     constexpr int N = Logits<T>::N, kChunk = PACKS * kRowThreads;
     __shared__ uint64_t list[kListMax];
-    __shared__ FloorShared<uint32_t> sh_floor[2];
+    __shared__ uint4 packs[kPackMax];
+    __shared__ int pack_token[kPackMax];
+    __shared__ FloorShared sh_floor[2];
     __shared__ double sh_sum[kRowWarps];
     __shared__ int sh_ref[kRowWarps];
     __shared__ uint32_t sh_top[kRowWarps];
-    __shared__ int sh_n, sh_odd;
+    __shared__ int sh_packs, sh_n, sh_odd;
     const int64_t r = blockIdx.x / p.splits;
     const int s = blockIdx.x % p.splits;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if ((p.finished && p.finished[r]) || !isfinite(p.cum[r])) return;
-    if (threadIdx.x == 0) { sh_n = 0; sh_odd = 0; }
+    if (threadIdx.x == 0) { sh_packs = 0; sh_n = 0; sh_odd = 0; }
     const T* row = static_cast<const T*>(p.logits) + r * p.stride;
     // packs are counted from the 16-byte boundary at or below the row's start
     const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
@@ -334,17 +343,17 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
             start + (c + 1) * kChunk * N <= p.vocab) {
 #pragma unroll
             for (int q = 0; q < PACKS; ++q)
-                v[q].raw = *reinterpret_cast<const uint4*>(row + token_of(c, q));
+                v[q].raw = __ldcs(reinterpret_cast<const uint4*>(row + token_of(c, q)));
             return;
         }
 #pragma unroll
         for (int q = 0; q < PACKS; ++q) {
             const int e = token_of(c, q);
-            if ((c * PACKS + q) * kRowThreads + static_cast<int>(threadIdx.x) >= p.per_split || e >= p.vocab) {
-                v[q].fill(neg_inf());
-            } else if (e >= 0 && e + N <= p.vocab) {
-                v[q].raw = *reinterpret_cast<const uint4*>(row + e);
-            } else {
+            const bool mine = (c * PACKS + q) * kRowThreads + static_cast<int>(threadIdx.x) < p.per_split;
+            v[q].fill(neg_inf());
+            if (mine && e >= 0 && e + N <= p.vocab) {
+                v[q].raw = __ldcs(reinterpret_cast<const uint4*>(row + e));
+            } else if (mine && e < p.vocab) {           // an end of the row
                 T t[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i)
@@ -354,8 +363,6 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
         }
     };
     const int chunks = (p.per_split + kChunk - 1) / kChunk;
-    Logits<T> next[PACKS];
-    load(0, next);
     float best = neg_inf(), floor_x = 0.0f;
     uint32_t floor_b = 0;
     double sum = 0.0;
@@ -364,10 +371,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
     int turn = 0;
     for (int c = 0; c < chunks; ++c) {
         Logits<T> v[PACKS];
-#pragma unroll
-        for (int q = 0; q < PACKS; ++q) v[q] = next[q];
-        if (c + 1 < chunks) load(c + 1, next);
-        else grid_release();
+        load(c, v);
+        if (c + 1 == chunks) grid_release();
         float most[PACKS], m = neg_inf();
 #pragma unroll
         for (int q = 0; q < PACKS; ++q) {
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
                 any = true;
             }
             const float2 l2 = make_float2(kLog2e, kLog2e), shift = make_float2(-ref, -ref);
-            double chunk = 0.0;
+            float chunk = 0.0f;
 #pragma unroll
             for (int q = 0; q < PACKS; ++q) {
                 float2 part = make_float2(0.0f, 0.0f);
@@ -394,12 +399,12 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
                     const float2 t = fma2(v[q].pair(i), l2, shift);
                     part = add2(part, make_float2(exp2_fast(t.x), exp2_fast(t.y)));
                 }
-                chunk += static_cast<double>(part.x + part.y);
+                chunk += part.x + part.y;
             }
-            sum += chunk;
+            sum += static_cast<double>(chunk);
             odd |= chunk != chunk;      // NaN among the logits
         }
-        if ((c & (c + 1)) == 0 || c + 1 == chunks) {
+        if (c == 0 || c == 3 || c + 1 == chunks) {
             floor_b = block_floor(choice_key(best), p.k, p.rounds, sh_floor[turn & 1]);
             ++turn;
             // everything above -inf where fewer than k were seen
@@ -407,15 +412,11 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
         }
 #pragma unroll
         for (int q = 0; q < PACKS; ++q) {
-            if (!(most[q] >= floor_x)) continue;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float x = v[q].at(i);
-                if (x >= floor_x) {
-                    const int at = atomicAdd(&sh_n, 1);
-                    if (at < kListMax)
-                        list[at] = (static_cast<uint64_t>(choice_key(x)) << 32) |
-                                   (0xffffffffu - static_cast<uint32_t>(token_of(c, q) + i));
+            if (most[q] >= floor_x) {
+                const int at = shared_add(&sh_packs, 1);
+                if (at < kPackMax) {
+                    packs[at] = v[q].raw;
+                    pack_token[at] = token_of(c, q);
                 }
             }
         }
@@ -440,24 +441,42 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const Beam
         top = max(top, sh_top[w]);
         ref_b = max(ref_b, sh_ref[w]);
     }
-    const int n = sh_n;
-    if (sh_odd || n > kListMax || (top != 0u && key_value(top) < kLow)) {
-        const int from = max(start, 0);
-        const int to = static_cast<int>(min(static_cast<int64_t>(start) + static_cast<int64_t>(p.per_split) * N,
-                                            static_cast<int64_t>(p.vocab)));
-        segment_exact(p, row, from, to, blockIdx.x, list);
-        return;
-    }
-    if (threadIdx.x == 0) {
+    const bool wild = sh_odd || (top != 0u && key_value(top) < kLow);
+    if (!wild && threadIdx.x == 0) {
         double total = 0.0;
         for (int w = 0; w < kRowWarps; ++w) total += scale_down(sh_sum[w], sh_ref[w] - ref_b);
         p.part_ref[blockIdx.x] = top == 0u ? static_cast<double>(neg_inf()) : ref_b * kLn2;
         p.part_sum[blockIdx.x] = total;
     }
+    const int n_packs = sh_packs;
+    if (!wild && n_packs <= kPackMax) {
+        for (int i = threadIdx.x; i < n_packs; i += kRowThreads) {
+            Logits<T> v;
+            v.raw = packs[i];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float x = v.at(j);
+                if (x >= floor_x) {
+                    const int at = shared_add(&sh_n, 1);
+                    if (at < kListMax)
+                        list[at] = (static_cast<uint64_t>(choice_key(x)) << 32) |
+                                   (0xffffffffu - static_cast<uint32_t>(pack_token[i] + j));
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int n = sh_n;
+    if (wild || n_packs > kPackMax || n > kListMax) {
+        const int from = max(start, 0);
+        const int to = static_cast<int>(min(static_cast<int64_t>(start) + static_cast<int64_t>(p.per_split) * N,
+                                            static_cast<int64_t>(p.vocab)));
+        segment_exact(p, row, from, to, blockIdx.x, wild, list);
+        return;
+    }
     uint64_t* out = p.cand + static_cast<int64_t>(blockIdx.x) * p.k;
-    const uint64_t least = static_cast<uint64_t>(floor_b) << 32;
-    rank_into(n, p.k, [&](int i) { return list[i] >= least; },
-              [&](int j, int i) { return list[j] > list[i]; }, [&](int rank, int i) { out[rank] = list[i]; });
+    rank_into(n, p.k, [&](int j, int i) { return list[j] > list[i]; },
+              [&](int rank, int i) { out[rank] = list[i]; });
     for (int j = n + threadIdx.x; j < p.k; j += kRowThreads) out[j] = 0;
 }
 
@@ -469,42 +488,62 @@ __device__ __forceinline__ bool better(const Choice& a, const Choice& b) {
     return a.key > b.key || (a.key == b.key && a.at < b.at);
 }
 
-// One sequence: its beams' sums, then the k best of the chunks' candidates.
+// One sequence: its beams' sums, then the k best of the segments' candidates.  Few
+// blocks run, so the time is the chain of loads and exchanges: all loads start
+// together, and the first kHeld candidates of a thread stay in registers.
 template <class T>
-__global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_constant__ BeamParams p) {
     __shared__ double sh_base[kMaxBeams];       // cum - log sum exp(x - ref); NaN: no candidates
     __shared__ double sh_ref[kMaxBeams];
     __shared__ float sh_off[kMaxBeams];         // error of that
     __shared__ int sh_redo[kMaxBeams];
     __shared__ Choice list[kListMax];
     __shared__ Choice best[kMaxBeamK];
-    __shared__ FloorShared<uint64_t> sh_floor;
+    __shared__ FloorShared sh_floor;
     __shared__ double sh_sum[kRowWarps];
     __shared__ float sh_err;
     __shared__ int sh_n, sh_again;
     const int64_t b = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per_beam = p.splits * p.k, total = p.beams * per_beam;
+    const uint64_t* cand = p.cand + b * total;
+    int lanes = 1;              // lanes that hold a segment's sum
+    while (lanes < 32 && lanes < p.splits) lanes *= 2;
+    // a warp takes every 8th candidate, of all beams: the floor is the better, the more
+    // evenly the best ones lie over the warps
+    const int first = lane * kRowWarps + warp;
     grid_wait();
+    uint64_t held[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int i = j * kRowThreads + first;
+        held[j] = i < total ? cand[i] : 0;
+    }
     for (int w = warp; w < p.beams; w += kRowWarps) {
         const int64_t r = b * p.beams + w;
+        const double none = static_cast<double>(neg_inf());
+        double f = none, part = 0.0;
+        if (lane < p.splits) {
+            f = p.part_ref[r * p.splits + lane];
+            part = p.part_sum[r * p.splits + lane];
+        }
         const float cum = p.cum[r];
         const bool done = p.finished && p.finished[r];
         double base = __longlong_as_double(0x7ff8000000000000ll), sum = 0.0;
-        const double none = static_cast<double>(neg_inf());
         double ref = none;
-        if (isfinite(cum) && !done) {
-            for (int s = lane; s < p.splits; s += 32) ref = fmax(ref, p.part_ref[r * p.splits + s]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ref = fmax(ref, __shfl_xor_sync(kFullMask, ref, o));
+        if (isfinite(cum) && !done) {       // else its segments wrote nothing
+            ref = f;
+            for (int s = lane + 32; s < p.splits; s += 32) ref = fmax(ref, p.part_ref[r * p.splits + s]);
+            for (int o = lanes / 2; o > 0; o >>= 1) ref = fmax(ref, __shfl_xor_sync(kFullMask, ref, o));
+            ref = __shfl_sync(kFullMask, ref, 0);
             for (int s = lane; s < p.splits; s += 32) {
-                const double f = p.part_ref[r * p.splits + s];
-                if (f > none) {
-                    const double part = p.part_sum[r * p.splits + s];
-                    sum += f == ref ? part : part * exp(f - ref);
+                if (s != lane) {
+                    f = p.part_ref[r * p.splits + s];
+                    part = p.part_sum[r * p.splits + s];
                 }
+                if (f > none) sum += f == ref ? part : part * exp(f - ref);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+            for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
             if (ref > none) base = static_cast<double>(cum) - log(sum);
         } else if (isfinite(cum)) {
             base = cum;
@@ -518,9 +557,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParam
             sh_redo[w] = 0;
         }
     }
-    const int per_beam = p.splits * p.k, total = p.beams * per_beam;
-    const uint64_t* cand = p.cand + b * total;
-    auto choice_of = [&](int i) {
+    auto choice_of = [&](int i, uint64_t v) {
         Choice c{0, 0};
         const int w = i / per_beam;
         const double base = sh_base[w];
@@ -533,7 +570,6 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParam
             }
             return c;
         }
-        const uint64_t v = cand[i];
         const uint32_t key = static_cast<uint32_t>(v >> 32);
         if (key == 0u) return c;
         const float x = key_value(key);
@@ -543,38 +579,46 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParam
         else if (x == -neg_inf()) c.key = choice_key(base);
         return c;
     };
+    // fn(choice) for every candidate of the thread
+    auto each = [&](auto&& fn) {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = j * kRowThreads + first;
+            if (i < total) fn(choice_of(i, held[j]));
+        }
+        for (int i = kHeld * kRowThreads + first; i < total; i += kRowThreads) fn(choice_of(i, cand[i]));
+    };
     for (int attempt = 0; ; ++attempt) {
         __syncthreads();
-        if (threadIdx.x == 0) {
-            sh_n = 0;
-            sh_again = 0;
-            float e = 0.0f;
-            for (int w = 0; w < p.beams; ++w) e = fmaxf(e, sh_off[w]);
-            sh_err = 2.0f * e;
+        if (warp == 0) {
+            float e = fmaxf(lane < p.beams ? sh_off[lane] : 0.0f, lane + 32 < p.beams ? sh_off[lane + 32] : 0.0f);
+            e = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(e)));
+            if (lane == 0) {
+                sh_n = 0;
+                sh_again = 0;
+                sh_err = 2.0f * e;
+            }
         }
         uint64_t mine = 0;
-        for (int i = threadIdx.x; i < total; i += kRowThreads) {
-            const uint64_t key = choice_of(i).key;
-            mine = key > mine ? key : mine;
-        }
-        uint64_t floor_b = block_floor(mine, p.k, p.rounds, sh_floor);
-        // a key below the floor by less than the sums' error could belong above it
-        if (floor_b != 0) floor_b = choice_key(key_value(floor_b) - static_cast<double>(sh_err));
+        each([&](const Choice& c) { mine = c.key > mine ? c.key : mine; });
+        // a floor in fp32, rounded down, and lower by the sums' error: a key that much
+        // below could belong above
+        const uint32_t floor_f = block_floor(choice_key(__double2float_rd(key_value(mine))), p.k, p.rounds, sh_floor);
+        uint64_t floor_b = 1;
+        if (floor_f != 0u) floor_b = choice_key(static_cast<double>(key_value(floor_f)) - static_cast<double>(sh_err));
         if (floor_b == 0) floor_b = 1;
         if (mine >= floor_b) {
-            for (int i = threadIdx.x; i < total; i += kRowThreads) {
-                const Choice c = choice_of(i);
-                if (c.key < floor_b) continue;
-                const int at = atomicAdd(&sh_n, 1);
+            each([&](const Choice& c) {
+                if (c.key < floor_b) return;
+                const int at = shared_add(&sh_n, 1);
                 if (at < kListMax) list[at] = c;
-            }
+            });
         }
         for (int j = threadIdx.x; j < p.k; j += kRowThreads) best[j] = Choice{0, 0};
         __syncthreads();
         const int n = min(sh_n, kListMax);
         if (sh_n <= kListMax) {
-            rank_into(n, p.k, [](int) { return true; },
-                      [&](int j, int i) { return better(list[j], list[i]); },
+            rank_into(n, p.k, [&](int j, int i) { return better(list[j], list[i]); },
                       [&](int rank, int i) { best[rank] = list[i]; });
             __syncthreads();
         } else {
@@ -582,10 +626,9 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParam
             Choice last{~0ull, 0};
             for (int j = 0; j < p.k; ++j) {
                 Choice c{0, 0};
-                for (int i = threadIdx.x; i < total; i += kRowThreads) {
-                    const Choice x = choice_of(i);
+                each([&](const Choice& x) {
                     if (x.key != 0 && better(last, x) && better(x, c)) c = x;
-                }
+                });
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
                     Choice x;
@@ -623,10 +666,9 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const BeamParam
             for (int i = threadIdx.x; i < n; i += kRowThreads)
                 if (better(last, list[i])) close(last, list[i]);
         } else {
-            for (int i = threadIdx.x; i < total; i += kRowThreads) {
-                const Choice c = choice_of(i);
+            each([&](const Choice& c) {
                 if (better(last, c)) close(last, c);
-            }
+            });
         }
         __syncthreads();
         if (!sh_again) break;
@@ -719,11 +761,11 @@ cudaError_t launch_reorder(const ReorderParams& p, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// How rows are cut.  A block holds 4 packs of 16 bytes a thread at a time (16 KB) and
+// How rows are cut.  A block holds 8 packs of 16 bytes a thread at a time (32 KB) and
 // runs through its segment.  Where all segments of one chunk would not fill the
-// machine twice, chunks shrink to 2 or 1 packs a thread, for more blocks.  Else
-// the segments are as long as leaves the fewest chunks in a row on a slot (4 blocks an
-// SM), each segment counting 1.5 more for its floor, list and results.
+// machine twice, chunks shrink to 4, 2 or 1 packs a thread, for more blocks.  Else
+// the segments are as long as leaves the busiest SM the fewest chunks, each segment
+// counting one more for its floors, lists and results.
 struct BeamPlan {
     int packs, splits, per_split;
     size_t cand, sum, ref, end;
@@ -735,13 +777,13 @@ BeamPlan beam_plan(const mflat_cu_beam_t* b, int batch) {
     const int64_t row_packs = (static_cast<int64_t>(b->vocab) + 2 * (n - 1)) / n;
     auto chunks_of = [&](int packs) { return (row_packs + packs * kRowThreads - 1) / (packs * kRowThreads); };
     BeamPlan p{};
-    p.packs = 4;
+    p.packs = 8;
     while (p.packs > 1 && rows * chunks_of(p.packs) < 2 * 148) p.packs /= 2;
-    const int64_t chunks = chunks_of(p.packs), slots = 4 * 148;
+    const int64_t chunks = chunks_of(p.packs);
     double least = 1e300;
     for (int64_t s = 1; s <= chunks; ++s) {
-        const double cost = static_cast<double>((rows * s + slots - 1) / slots) *
-                            (static_cast<double>((chunks + s - 1) / s) + 1.5);
+        const double cost = static_cast<double>((rows * s + 147) / 148) *
+                            (static_cast<double>(chunks) / static_cast<double>(s) + 1.0);
         if (cost < least) {
             least = cost;
             p.splits = static_cast<int>(s);
@@ -838,7 +880,8 @@ extern "C" int mflat_cu_beam_select(const mflat_cu_beam_t* b, const void* logits
         switch (l.packs) {
             case 1: beam_segment_kernel<T, 1><<<grid, kRowThreads, 0, st>>>(p); break;
             case 2: beam_segment_kernel<T, 2><<<grid, kRowThreads, 0, st>>>(p); break;
-            default: beam_segment_kernel<T, 4><<<grid, kRowThreads, 0, st>>>(p); break;
+            case 4: beam_segment_kernel<T, 4><<<grid, kRowThreads, 0, st>>>(p); break;
+            default: beam_segment_kernel<T, 8><<<grid, kRowThreads, 0, st>>>(p); break;
         }
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
