@@ -7,6 +7,12 @@
 // fp32, whose error is below tau, and takes the selection when every gap between
 // neighbours in it (and at the cut between kept and dropped groups) exceeds
 // tau; the other tokens are selected again from scores in 64 bits.
+//
+// Lists.  The tokens are cut into tiles, one block each.  A block ranks its choices
+// among those of the same expert in its tile (in order: warps own adjacent choices
+// and count in histograms of their own) and leaves its count per expert; a second
+// kernel sums the counts of the tiles before and scatters.  Nothing depends on
+// the order in which blocks run.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -29,7 +35,9 @@ int operator_device(int device, int* out) {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxRouteK = 32, kMaxGroups = 32;
-constexpr int kRouteThreads = 256;
+constexpr int kGradThreads = 256;
+constexpr int kCandMax = 64;        // candidates of a token that one warp ranks
+constexpr int kTiles = 148;         // one tile an SM
 
 struct RouteParams {
     const void* logits;
@@ -42,6 +50,13 @@ struct RouteParams {
     const uint8_t* mask;
     int32_t* ids;
     float* weights;
+    int lane_groups;            // lanes that share a group where that is a power of two, else 0
+    // lists
+    int tiles, tile;            // tokens per tile
+    uint16_t* ranks;            // workspace [tokens * k]: rank among the tile's choices of the expert
+    uint16_t* counts;           // workspace [tiles][experts rounded up to 2]
+    int32_t* start;
+    int32_t* slots;
 };
 
 // Error bounds of an fp32 choice score and of a sum of two.  The scores are in
@@ -105,21 +120,21 @@ __device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S
     }
 }
 
-// Group selection: clears the keys of experts outside the groups_kept best
-// groups.  Returns whether a gap at the cut is too small for fp32.
-template <class S, int LPT, int VPL, class K>
-__device__ __forceinline__ bool keep_groups(const RouteParams& p, int lane, const S (&c)[VPL],
-                                            K (&key)[VPL]) {
+// Each group's score, group by group over all lanes, for any group size: lane g
+// gets the score of group g; tau the bound of the sums' errors.
+template <class S, int LPT, int VPL>
+__device__ __forceinline__ S group_scores(const RouteParams& p, int lane, const S (&c)[VPL],
+                                          const bool (&in)[VPL], float& tau) {
     const S none = S(neg_inf());
     const int size = p.experts / p.groups;
-    S mine = none;              // lane g: score of group g
-    float tau = 0.0f;
+    S mine = none;
+    tau = 0.0f;
     for (int g = 0; g < p.groups; ++g) {
         S a = none, b = none;   // the group's two largest
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             const int e = lane * VPL + j;
-            if (e >= g * size && e < (g + 1) * size && key[j] != 0) {
+            if (e >= g * size && e < (g + 1) * size && in[j]) {
                 const S v = c[j];
                 if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
             }
@@ -135,43 +150,32 @@ __device__ __forceinline__ bool keep_groups(const RouteParams& p, int lane, cons
         if (lane == g) mine = two ? a + b : a;
         if (a != none) tau = fmaxf(tau, tau_of(float(a)) + (two ? tau_of(float(b)) : 0.0f));
     }
-    // a group's rank among all (ties to the lower group)
+    return mine;
+}
+
+// The groups that stay, as bits: lane g holds the score of group g.  Ties to the
+// lower group.
+template <class S, int LPT>
+__device__ __forceinline__ unsigned kept_groups(const RouteParams& p, int lane, S mine) {
     int rank = 0;
     const int base = (threadIdx.x & 31) - lane;
     for (int g = 0; g < p.groups; ++g) {
         const S v = __shfl_sync(kFullMask, mine, base + g);
         rank += (v > mine || (v == mine && g < lane)) ? 1 : 0;
     }
-    const bool kept = lane < p.groups && rank < p.groups_kept;
-    const unsigned all = __ballot_sync(kFullMask, kept);
-    const unsigned bits = (all >> base) & (LPT == 32 ? kFullMask : (1u << (LPT & 31)) - 1u);
-    bool doubt = false;
-    if constexpr (sizeof(S) == 4) {
-        const uint32_t cut = lane_max<LPT>(lane < p.groups && !kept ? choice_key(mine) : 0u);
-        const uint32_t low = ~lane_max<LPT>(kept ? ~choice_key(mine) : 0u);
-        if (cut != 0u && low != 0u) doubt = !(key_value(low) - key_value(cut) > tau);
-    }
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-        const int g = min((lane * VPL + j) / size, 31);
-        if (!((bits >> g) & 1u)) key[j] = 0;
-    }
-    return doubt;
+    const unsigned all = __ballot_sync(kFullMask, lane < p.groups && rank < p.groups_kept);
+    return (all >> base) & (LPT == 32 ? kFullMask : (1u << (LPT & 31)) - 1u);
 }
 
 // The k largest keys, ties to the lowest expert: lane r of the token gets the
-// r-th expert (or -1) and its logit.  With `check`, returns whether a gap in the
-// selection is too small for fp32 scores.
+// r-th expert (or -1) and its logit.
 template <int LPT, int VPL, class K>
-__device__ __forceinline__ bool take_best(K (&key)[VPL], const float (&x)[VPL], int k, int lane,
-                                          bool check, int& id, float& xid) {
+__device__ __forceinline__ void take_best(K (&key)[VPL], const float (&x)[VPL], int k, int lane,
+                                          int& id, float& xid) {
     const int base = (threadIdx.x & 31) - lane;
     id = -1;
     xid = neg_inf();
-    bool doubt = false;
-    K before = 0;
-    const int rounds = check ? k + 1 : k;
-    for (int r = 0; r < rounds; ++r) {
+    for (int r = 0; r < k; ++r) {
         K best = 0;
         int at = 0;
         float xb = 0.0f;
@@ -184,21 +188,13 @@ __device__ __forceinline__ bool take_best(K (&key)[VPL], const float (&x)[VPL], 
         const int src = __ffs(who) - 1;
         const int e = __shfl_sync(kFullMask, lane * VPL + at, base + src);
         xb = __shfl_sync(kFullMask, xb, base + src);
-        if (lane == r && r < k && top != 0) { id = e; xid = xb; }
+        if (lane == r && top != 0) { id = e; xid = xb; }
         if (lane == src) {
 #pragma unroll
             for (int j = 0; j < VPL; ++j)
                 if (j == at) key[j] = 0;
         }
-        if constexpr (sizeof(K) == 4) {
-            if (check && r > 0 && top != 0) {
-                const float hi = key_value(before), lo = key_value(top);
-                if (!(hi - lo > tau_of(hi))) doubt = true;
-            }
-        }
-        before = top;
     }
-    return doubt;
 }
 
 // Weights of the chosen experts: lane r holds the r-th one's logit.  Plain:
@@ -252,116 +248,406 @@ __device__ __forceinline__ void load_row(const RouteParams& p, int64_t t, int la
         if (!(x[j] > neg_inf())) x[j] = neg_inf();
 }
 
-// LPT lanes per token, VPL experts per lane.
+// A token from scores in 64 bits, for any values: the row is read again, so that the
+// common path keeps its registers.  Every lane of the warp calls it.
 template <class T, int LPT, int VPL>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
-    const int lane = threadIdx.x % LPT;
-    const int64_t t = (static_cast<int64_t>(blockIdx.x) * kRouteThreads + threadIdx.x) / LPT;
-    const bool live = t < p.tokens && (!p.mask || p.mask[t] != 0);
+__device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int lane, bool live,
+                                         int& id, float& xid) {
     float x[VPL];
     load_row<T, LPT, VPL>(p, t, lane, live, x);
-
-    // the row's maximum and sum, for softmax weights
-    float m = 0.0f, sum = 1.0f;
-    if (p.softmax && !p.renormalise) {
-        m = neg_inf();
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
-#pragma unroll
-        for (int o = LPT / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-        sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            sum += x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : __expf(x[j] - m);
-        sum = lane_sum<LPT>(sum);
-    }
-
-    float b[VPL];
-    if (p.bias) {
+    uint64_t key[VPL];
+    if (p.bias || (p.groups > 1 && p.group_top == 2)) {
+        double c[VPL];
+        bool in[VPL];
+        scores_of<double, LPT, VPL>(x, p.softmax, c);
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             const int e = lane * VPL + j;
-            b[j] = e < p.experts ? p.bias[e] : 0.0f;
+            if (p.bias && e < p.experts) c[j] += static_cast<double>(p.bias[e]);
+            key[j] = x[j] == neg_inf() ? 0ull : choice_key(p.bias ? c[j] : static_cast<double>(x[j]));
+            in[j] = key[j] != 0;
+        }
+        if (p.groups > 1) {
+            float unused;
+            const unsigned kept = kept_groups<double, LPT>(
+                p, lane, group_scores<double, LPT, VPL>(p, lane, c, in, unused));
+            const int size = p.experts / p.groups;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (!((kept >> min((lane * VPL + j) / size, 31)) & 1u)) key[j] = 0;
+        }
+    } else {
+        bool in[VPL];
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            key[j] = choice_key(static_cast<double>(x[j]));
+            in[j] = key[j] != 0;
+        }
+        if (p.groups > 1) {
+            float unused;
+            const unsigned kept = kept_groups<float, LPT>(
+                p, lane, group_scores<float, LPT, VPL>(p, lane, x, in, unused));
+            const int size = p.experts / p.groups;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (!((kept >> min((lane * VPL + j) / size, 31)) & 1u)) key[j] = 0;
         }
     }
-    const bool by_sums = p.groups > 1 && (p.bias || p.group_top == 2);
-    int id;
-    float xid;
+    take_best<LPT, VPL>(key, x, p.k, lane, id, xid);
+}
+
+// The groups' part of the choice in fp32: -inf for experts outside the kept ones.
+// Returns whether the cut is too close for fp32 (exact: c are logits, no doubt but
+// ties, which go to the lower group).  Where a group is 2^n lanes of a warp, their
+// top two meet in n exchanges, and each group is compared with all others: kept for
+// sure, dropped for sure, or in doubt.
+template <int LPT, int VPL>
+__device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, const float (&c)[VPL],
+                                              bool exact, float (&key)[VPL]) {
+    const float none = neg_inf();
+    if (p.lane_groups == 0) {
+        bool in[VPL];
+        float tau;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) in[j] = key[j] > none;
+        const float mine = group_scores<float, LPT, VPL>(p, lane, c, in, tau);
+        const unsigned kept = kept_groups<float, LPT>(p, lane, mine);
+        const int size = p.experts / p.groups;
+        const bool here = lane < p.groups && ((kept >> lane) & 1u);
+        float low = here ? mine : -none, cut = lane < p.groups && !here ? mine : none;
+#pragma unroll
+        for (int o = LPT / 2; o > 0; o >>= 1) {
+            low = fminf(low, __shfl_xor_sync(kFullMask, low, o));
+            cut = fmaxf(cut, __shfl_xor_sync(kFullMask, cut, o));
+        }
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+            if (!((kept >> min((lane * VPL + j) / size, 31)) & 1u)) key[j] = none;
+        return !exact && cut > none && !(low - cut > tau);
+    }
+    float a = none, b = none;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const float v = key[j] > none ? c[j] : none;
+        b = fmaxf(b, fminf(a, v));
+        a = fmaxf(a, v);
+    }
+    for (int o = 1; o < p.lane_groups; o <<= 1) {
+        const float a2 = __shfl_xor_sync(kFullMask, a, o), b2 = __shfl_xor_sync(kFullMask, b, o);
+        b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+        a = fmaxf(a, a2);
+    }
+    const bool two = p.group_top == 2 && b > none;
+    const float mine = two ? a + b : a;
+    float tau = a > none ? tau_of(a) + (two ? tau_of(b) : 0.0f) : 0.0f;
+#pragma unroll
+    for (int o = LPT / 2; o > 0; o >>= 1) tau = fmaxf(tau, __shfl_xor_sync(kFullMask, tau, o));
+    if (exact) tau = 0.0f;
+    const int base = (threadIdx.x & 31) - lane;
+    const int group = lane / p.lane_groups;
+    int above = 0, near = 0;    // groups above for sure, and those not below for sure
+    for (int g = 0; g < p.groups; ++g) {
+        const float v = __shfl_sync(kFullMask, mine, base + g * p.lane_groups);
+        const bool tie = v == mine && g < group;
+        above += (exact ? v > mine || tie : v > mine + tau) ? 1 : 0;
+        near += (g != group && (exact ? v > mine || tie : !(v < mine - tau))) ? 1 : 0;
+    }
+    const bool kept = near < p.groups_kept, dropped = above >= p.groups_kept || mine == none;
+    if (!kept) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) key[j] = none;
+    }
+    return group < p.groups && !kept && !dropped;
+}
+
+// A warp's scratch for one token's candidates.
+struct RouteScratch {
+    float2 cand[kCandMax];              // key, expert
+    float2 best[kMaxRouteK + 1];
+};
+
+// The k largest fp32 keys of a token that a whole warp holds (VPL > 1).  The k-th
+// largest lane maximum is a floor that few keys reach; those are ranked by counting.
+// Lane r gets the r-th expert, or -1.  Returns whether it has to be done exactly: with
+// `check` where neighbours are too close for fp32, and for more candidates than fit.
+template <int VPL>
+__device__ __forceinline__ bool take_best_warp(const float (&key)[VPL], int k, bool check,
+                                               RouteScratch& sh, int& id) {
+    const int lane = threadIdx.x & 31;
+    const int want = min(k + (check ? 1 : 0), 32);
+    float top = key[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) top = fmaxf(top, key[j]);
+    float v = top;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float w = __shfl_xor_sync(kFullMask, v, o);
+            const bool larger = ((lane & size) == 0) == ((lane & o) == 0);
+            v = larger ? fmaxf(v, w) : fminf(v, w);
+        }
+    const float floor_v = __shfl_sync(kFullMask, v, want - 1);
+    const unsigned below = (1u << lane) - 1u;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const bool in = key[j] >= floor_v && key[j] > neg_inf();
+        const unsigned who = __ballot_sync(kFullMask, in);
+        const int at = n + __popc(who & below);
+        if (in && at < kCandMax) sh.cand[at] = make_float2(key[j], __int_as_float(lane * VPL + j));
+        n += __popc(who);
+    }
+    if (n > kCandMax) return true;
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        const float2 c = sh.cand[i];
+        const int e = __float_as_int(c.y);
+        int rank = 0;
+        for (int m = 0; m < n; ++m) {
+            const float2 d = sh.cand[m];
+            rank += d.x > c.x || (d.x == c.x && __float_as_int(d.y) < e) ? 1 : 0;
+        }
+        if (rank <= k) sh.best[rank] = c;
+    }
+    __syncwarp();
+    const float2 mine = lane < n && lane <= k ? sh.best[lane] : make_float2(neg_inf(), 0.0f);
+    id = lane < k && lane < n ? __float_as_int(mine.y) : -1;
     bool doubt = false;
-    {
-        uint32_t key[VPL];
-        if (p.bias || by_sums) {
+    if (check) {
+        // lane k holds the first that stays out (k = 32: look it up)
+        float next = __shfl_down_sync(kFullMask, mine.x, 1);
+        if (lane == 31) next = k == 32 && n > 32 ? sh.best[32].x : neg_inf();
+        doubt = lane < k && next > neg_inf() && !(mine.x - next > tau_of(mine.x));
+        // 32 lane maxima vouch for 32 candidates, not for the one after
+        doubt |= k == 32 && n <= 32;
+    }
+    __syncwarp();
+    return __any_sync(kFullMask, doubt);
+}
+
+// Exclusive sums of one value per thread's run over the block's values v[0, n) in
+// shared memory, in place; returns nothing.  n <= 1024.
+template <int NT>
+__device__ __forceinline__ void block_exclusive(int* v, int n, int* warp_sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (n + NT - 1) / NT, i0 = threadIdx.x * per;
+    int sum = 0;
+    for (int i = 0; i < per; ++i) sum += i0 + i < n ? v[i0 + i] : 0;
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFullMask, incl, o);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int s = lane < NT / 32 ? warp_sum[lane] : 0;
+        const int own = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(kFullMask, s, o);
+            if (lane >= o) s += u;
+        }
+        if (lane < NT / 32) warp_sum[lane] = s - own;
+    }
+    __syncthreads();
+    int run = warp_sum[warp] + incl - sum;
+    for (int i = 0; i < per; ++i)
+        if (i0 + i < n) {
+            const int c = v[i0 + i];
+            v[i0 + i] = run;
+            run += c;
+        }
+    __syncthreads();
+}
+
+// One tile of tokens a block, LPT lanes per token, VPL experts per lane.  With lists,
+// then the ranks of the tile's choices and its counts; one tile alone goes all the way.
+template <class T, int LPT, int VPL, int NT>
+__global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ RouteParams p) {
+    constexpr int kWarps = NT / 32, kAtOnce = NT / LPT, kMost = LPT * VPL;
+    __shared__ RouteScratch scratch[VPL > 1 ? kWarps : 1];
+    const int lane = threadIdx.x % LPT, warp = threadIdx.x >> 5;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
+    const int64_t t1 = min(t0 + p.tile, static_cast<int64_t>(p.tokens));
+    const bool by_sums = p.bias || (p.groups > 1 && p.group_top == 2);
+    float b[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int e = lane * VPL + j;
+        b[j] = p.bias && e < p.experts ? p.bias[e] : 0.0f;
+    }
+    for (int64_t tb = t0 + warp * (32 / LPT); tb < t1; tb += kAtOnce) {
+        const int64_t t = tb + (threadIdx.x & 31) / LPT;
+        const bool live = t < t1 && (!p.mask || p.mask[t] != 0);
+        float x[VPL], key[VPL];
+        load_row<T, LPT, VPL>(p, t, lane, live, x);
+        // the row's maximum and sum, for softmax weights
+        float m = 0.0f, sum = 1.0f;
+        if (p.softmax && !p.renormalise) {
+            m = neg_inf();
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
+#pragma unroll
+            for (int o = LPT / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+            sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                sum += x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : __expf(x[j] - m);
+            sum = lane_sum<LPT>(sum);
+        }
+        bool doubt = false;
+        if (by_sums) {
             float c[VPL];
             scores_of<float, LPT, VPL>(x, p.softmax, c);
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                if (p.bias) c[j] += b[j];
-                key[j] = x[j] == neg_inf() ? 0u : choice_key(p.bias ? c[j] : x[j]);
+                c[j] += b[j];
+                key[j] = p.bias ? (x[j] > neg_inf() && c[j] > neg_inf() ? c[j] : neg_inf()) : x[j];
             }
-            if (p.groups > 1) doubt = keep_groups<float, LPT, VPL>(p, lane, c, key);
+            if (p.groups > 1) doubt = choose_groups<LPT, VPL>(p, lane, c, false, key);
         } else {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) key[j] = choice_key(x[j]);
-            if (p.groups > 1) keep_groups<float, LPT, VPL>(p, lane, x, key);   // exact: no doubt
+            for (int j = 0; j < VPL; ++j) key[j] = x[j];
+            if (p.groups > 1) choose_groups<LPT, VPL>(p, lane, x, true, key);
         }
-        doubt |= take_best<LPT, VPL>(key, x, p.k, lane, p.bias != nullptr, id, xid);
-    }
-    if (__any_sync(kFullMask, doubt)) {
-        uint64_t key[VPL];
-        double c[VPL];
-        scores_of<double, LPT, VPL>(x, p.softmax, c);
+        int id = -1;
+        float xid = neg_inf();
+        if constexpr (VPL > 1) {
+            doubt |= take_best_warp<VPL>(key, p.k, p.bias != nullptr, scratch[warp], id);
+        } else {
+            // one expert a lane: its rank by counting
+            const int base = (threadIdx.x & 31) - lane;
+            int rank = 0;
+            float next = neg_inf();     // the largest below
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            if (p.bias) c[j] += static_cast<double>(b[j]);
-            key[j] = x[j] == neg_inf() ? 0ull : choice_key(p.bias ? c[j] : static_cast<double>(x[j]));
+            for (int e = 0; e < LPT; ++e) {
+                const float v = __shfl_sync(kFullMask, key[0], base + e);
+                const bool before = v > key[0] || (v == key[0] && e < lane);
+                rank += before ? 1 : 0;
+                next = !before && e != lane ? fmaxf(next, v) : next;
+            }
+            if (!(key[0] > neg_inf())) rank = LPT;
+            if (p.bias && rank < p.k && next > neg_inf()) doubt |= !(key[0] - next > tau_of(key[0]));
+            for (int r = 0; r < p.k; ++r) {
+                const unsigned who = __ballot_sync(kFullMask, rank == r) >> base;
+                const unsigned own = LPT == 32 ? who : who & ((1u << (LPT & 31)) - 1u);
+                if (lane == r && own) id = __ffs(own) - 1;
+            }
         }
-        if (p.groups > 1) keep_groups<double, LPT, VPL>(p, lane, c, key);
-        take_best<LPT, VPL>(key, x, p.k, lane, false, id, xid);
+        if (__any_sync(kFullMask, doubt)) {
+            exact_token<T, LPT, VPL>(p, t, lane, live, id, xid);
+        } else if (id >= 0) {
+            xid = to_float(static_cast<const T*>(p.logits)[t * p.stride + id]);
+        }
+        const float w = weight_of<LPT>(p, id >= 0, xid, m, sum);
+        if (t < t1 && lane < p.k) {
+            p.ids[t * p.k + lane] = id;
+            p.weights[t * p.k + lane] = w;
+        }
     }
-    const float w = weight_of<LPT>(p, id >= 0, xid, m, sum);
-    if (t < p.tokens && lane < p.k) {
-        p.ids[t * p.k + lane] = id;
-        p.weights[t * p.k + lane] = w;
+    if (!p.start) return;
+
+    // ranks: warps own adjacent runs of the tile's choices
+    __shared__ uint16_t hist[kWarps][kMost];
+    __shared__ int total[kMost + 1];
+    __shared__ int warp_sum[32];
+    const int full_lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; i < kWarps * kMost / 2; i += NT) reinterpret_cast<uint32_t*>(&hist[0][0])[i] = 0;
+    __syncthreads();
+    grid_release();
+    const int64_t e0 = t0 * p.k, n = (t1 - t0) * p.k;
+    const int64_t run = (n + kWarps * 32 - 1) / (kWarps * 32) * 32;
+    const int64_t r0 = e0 + warp * run, r1 = min(r0 + run, e0 + n);
+    for (int64_t i0 = r0; i0 < r1; i0 += 32) {
+        const int64_t i = i0 + full_lane;
+        const int id = i < r1 ? p.ids[i] : -1;
+        const unsigned peers = __match_any_sync(kFullMask, id);
+        const int rank = __popc(peers & ((1u << full_lane) - 1u));
+        int before = 0;
+        if (id >= 0 && rank == 0) {
+            before = hist[warp][id];
+            hist[warp][id] = static_cast<uint16_t>(before + __popc(peers));
+        }
+        before = __shfl_sync(kFullMask, before, __ffs(peers) - 1);
+        if (id >= 0) p.ranks[i] = static_cast<uint16_t>(before + rank);
+        __syncwarp();
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.experts; e += NT) {
+        int s = 0;
+#pragma unroll 8
+        for (int w = 0; w < kWarps; ++w) {
+            const int c = hist[w][e];
+            hist[w][e] = static_cast<uint16_t>(s);
+            s += c;
+        }
+        total[e] = s;
+        if (p.tiles > 1) p.counts[static_cast<int64_t>(blockIdx.x) * ((p.experts + 1) & ~1) + e] = static_cast<uint16_t>(s);
+    }
+    if (p.tiles > 1) {
+        __syncthreads();
+        for (int64_t i = r0 + full_lane; i < r1; i += 32) {
+            const int id = p.ids[i];
+            if (id >= 0) p.ranks[i] = static_cast<uint16_t>(p.ranks[i] + hist[warp][id]);
+        }
+        return;
+    }
+    if (threadIdx.x == 0) total[p.experts] = 0;
+    __syncthreads();
+    block_exclusive<NT>(total, p.experts + 1, warp_sum);
+    for (int e = threadIdx.x; e <= p.experts; e += NT) p.start[e] = total[e];
+    for (int64_t i = r0 + full_lane; i < r1; i += 32) {
+        const int id = p.ids[i];
+        if (id >= 0) p.slots[total[id] + hist[warp][id] + p.ranks[i]] = static_cast<int32_t>(i);
     }
 }
 
-// Lists by expert, one block per expert: how many choices are below it, then
-// its own in order.
-__global__ void __launch_bounds__(256) lists_kernel(const int32_t* __restrict__ ids, int n,
-                                                    int experts, int32_t* start, int32_t* slots) {
-    __shared__ int sh[8], sh_base;
-    const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int below = 0;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int v = ids[i];
-        below += v >= 0 && v < e;
-    }
-    below = __reduce_add_sync(kFullMask, below);
-    if (lane == 0) sh[warp] = below;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int w = 0; w < 8; ++w) s += sh[w];
-        sh_base = s;
-        start[e] = s;
+// The lists of many tiles: where this tile's choices of each expert begin, then the
+// scatter.  A thread sums two adjacent experts over its share of the tiles' counts.
+constexpr int kListThreads = 1024;
+__global__ void __launch_bounds__(kListThreads) lists_kernel(const __grid_constant__ RouteParams p) {
+    __shared__ int before[kMaxExperts], total[kMaxExperts + 1];
+    __shared__ int warp_sum[32];
+    const int pairs = (p.experts + 1) / 2, groups = max(1, kListThreads / pairs);
+    for (int e = threadIdx.x; e <= p.experts; e += kListThreads) {
+        total[e] = 0;
+        if (e < p.experts) before[e] = 0;
     }
     __syncthreads();
-    int at = sh_base;
-    if (e == experts) return;
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int i = i0 + threadIdx.x;
-        const bool mine = i < n && ids[i] == e;
-        const unsigned b = __ballot_sync(kFullMask, mine);
-        if (lane == 0) sh[warp] = __popc(b);
-        __syncthreads();
-        int before = 0, all = 0;
-        for (int w = 0; w < 8; ++w) {
-            before += w < warp ? sh[w] : 0;
-            all += sh[w];
+    grid_wait();
+    const int pair = threadIdx.x % pairs, group = threadIdx.x / pairs;
+    if (group < groups) {
+        int b0 = 0, b1 = 0, s0 = 0, s1 = 0;
+        const uint32_t* rows = reinterpret_cast<const uint32_t*>(p.counts) + pair;
+#pragma unroll 8
+        for (int r = group; r < p.tiles; r += groups) {
+            const uint32_t c = rows[static_cast<int64_t>(r) * pairs];
+            const int lo = c & 0xffffu, hi = c >> 16;
+            s0 += lo;
+            s1 += hi;
+            b0 += r < static_cast<int>(blockIdx.x) ? lo : 0;
+            b1 += r < static_cast<int>(blockIdx.x) ? hi : 0;
         }
-        if (mine) slots[at + before + __popc(b & ((1u << lane) - 1u))] = i;
-        at += all;
-        __syncthreads();
+        // sums of whole numbers: the order of these additions changes nothing
+        atomicAdd(&before[2 * pair], b0);
+        atomicAdd(&total[2 * pair], s0);
+        if (2 * pair + 1 < p.experts) {
+            atomicAdd(&before[2 * pair + 1], b1);
+            atomicAdd(&total[2 * pair + 1], s1);
+        }
+    }
+    __syncthreads();
+    block_exclusive<kListThreads>(total, p.experts + 1, warp_sum);
+    if (blockIdx.x == 0)
+        for (int e = threadIdx.x; e <= p.experts; e += kListThreads) p.start[e] = total[e];
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
+    const int64_t t1 = min(t0 + p.tile, static_cast<int64_t>(p.tokens));
+    for (int64_t i = t0 * p.k + threadIdx.x; i < t1 * p.k; i += kListThreads) {
+        const int id = p.ids[i];
+        if (id >= 0) p.slots[total[id] + before[id] + p.ranks[i]] = static_cast<int32_t>(i);
     }
 }
 
@@ -370,11 +656,11 @@ __global__ void __launch_bounds__(256) lists_kernel(const int32_t* __restrict__ 
 // dx_e = scale * g_e s_e (1 - s_e).  Renormalised over the chosen (w = scale * s /
 // S): dx_j = w_j (g_j - sum_i g_i w_i / scale), for a sigmoid times 1 - s_j.
 template <class T, int LPT, int VPL>
-__global__ void __launch_bounds__(kRouteThreads)
+__global__ void __launch_bounds__(kGradThreads)
     route_backward_kernel(const RouteParams p, const float* __restrict__ grad, T* out,
                           int64_t out_stride) {
     const int lane = threadIdx.x % LPT, base = (threadIdx.x & 31) - lane;
-    const int64_t t = (static_cast<int64_t>(blockIdx.x) * kRouteThreads + threadIdx.x) / LPT;
+    const int64_t t = (static_cast<int64_t>(blockIdx.x) * kGradThreads + threadIdx.x) / LPT;
     const bool live = t < p.tokens;
     float x[VPL];
     load_row<T, LPT, VPL>(p, t, lane, live, x);
@@ -468,19 +754,20 @@ __global__ void __launch_bounds__(kRouteThreads)
     }
 }
 
-// Calls fn(LPT, VPL) as integral constants for a router: as few lanes per
-// token as hold its experts one each and its k choices.
+// Calls fn(LPT, VPL, NT) as integral constants for a router: as few lanes per
+// token as hold its experts one each and its k choices; blocks of one to an SM as
+// long as a thread's experts leave the registers for it.
 template <class Fn>
 cudaError_t with_layout(int experts, Fn&& fn) {
     using std::integral_constant;
-    if (experts <= 8) return fn(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    if (experts <= 16) return fn(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    if (experts <= 32) return fn(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    if (experts <= 64) return fn(integral_constant<int, 32>{}, integral_constant<int, 2>{});
-    if (experts <= 128) return fn(integral_constant<int, 32>{}, integral_constant<int, 4>{});
-    if (experts <= 256) return fn(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    if (experts <= 512) return fn(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-    return fn(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    if (experts <= 8) return fn(integral_constant<int, 8>{}, integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+    if (experts <= 16) return fn(integral_constant<int, 16>{}, integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+    if (experts <= 32) return fn(integral_constant<int, 32>{}, integral_constant<int, 1>{}, integral_constant<int, 1024>{});
+    if (experts <= 64) return fn(integral_constant<int, 32>{}, integral_constant<int, 2>{}, integral_constant<int, 1024>{});
+    if (experts <= 128) return fn(integral_constant<int, 32>{}, integral_constant<int, 4>{}, integral_constant<int, 1024>{});
+    if (experts <= 256) return fn(integral_constant<int, 32>{}, integral_constant<int, 8>{}, integral_constant<int, 1024>{});
+    if (experts <= 512) return fn(integral_constant<int, 32>{}, integral_constant<int, 16>{}, integral_constant<int, 512>{});
+    return fn(integral_constant<int, 32>{}, integral_constant<int, 32>{}, integral_constant<int, 256>{});
 }
 
 int pack_elems(int experts, size_t es) {   // elements of one load of load_row()
@@ -522,6 +809,27 @@ int check_router(const mflat_cu_router_t* r, int tokens) {
     return ST_OK;
 }
 
+// Tiles of the lists: one to an SM, no more tokens in one than 16-bit counts hold; up
+// to kOneTile tokens a single tile, whose block needs no second kernel.
+constexpr int kOneTile = 64;
+struct RoutePlan {
+    int tiles, tile;
+    size_t ranks, counts, end;
+};
+RoutePlan route_plan(const mflat_cu_router_t* r, int tokens) {
+    RoutePlan l{};
+    l.tiles = tokens <= kOneTile ? 1 : kTiles;
+    l.tile = (tokens + l.tiles - 1) / l.tiles;
+    if (l.tile > 65535) l.tile = 65535;
+    if (tokens > kOneTile && l.tile < 32) l.tile = 32;
+    l.tiles = (tokens + l.tile - 1) / l.tile;
+    auto round256 = [](size_t n) { return (n + 255) & ~size_t(255); };
+    l.ranks = 0;
+    l.counts = round256(static_cast<size_t>(tokens) * r->k * 2);
+    l.end = l.counts + round256(static_cast<size_t>(l.tiles) * ((r->experts + 1) & ~1) * 2);
+    return l;
+}
+
 int fill_params(const mflat_cu_router_t* r, const void* logits, int64_t& stride, int tokens,
                 RouteParams& p) {
     if (stride == 0) stride = r->experts;
@@ -540,6 +848,11 @@ int fill_params(const mflat_cu_router_t* r, const void* logits, int64_t& stride,
     p.group_top = r->group_top;
     p.scale = r->scale;
     p.vec = packed_rows(logits, stride, r->experts, type_bytes(r->type));
+    int vpl = 1;
+    while (vpl * 32 < r->experts) vpl *= 2;
+    const int size = r->experts / r->groups;
+    const int lanes = size % vpl == 0 ? size / vpl : 0;
+    p.lane_groups = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
     return ST_OK;
 }
 
@@ -549,9 +862,8 @@ int fill_params(const mflat_cu_router_t* r, const void* logits, int64_t& stride,
 using namespace mflat_cu;
 
 extern "C" size_t mflat_cu_route_workspace(const mflat_cu_router_t* r, int tokens) {
-    (void)r;
-    (void)tokens;
-    return 0;
+    if (check_router(r, tokens) != ST_OK || tokens == 0) return 0;
+    return route_plan(r, tokens).end;
 }
 
 extern "C" int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, int64_t stride,
@@ -567,6 +879,9 @@ extern "C" int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, in
         !aligned_to(start, 4) || !aligned_to(slots, 4))
         return fail(ST_BAD_ARG, "misaligned pointer");
     if (tokens == 0 && !start) return ST_OK;
+    const size_t need = start && tokens > 0 ? route_plan(r, tokens).end : 0;
+    if (need > 0 && (!ws || ws_bytes < need || !aligned_to(ws, 256)))
+        return fail(ST_BAD_ARG, "workspace missing, too small or not 256-byte aligned");
     rc = operator_device(device, &device);
     if (rc != ST_OK) return rc;
     DeviceGuard g(device);
@@ -579,19 +894,23 @@ extern "C" int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, in
     p.mask = mask;
     p.ids = ids;
     p.weights = weights;
+    const RoutePlan l = route_plan(r, tokens);
+    p.tiles = l.tiles;
+    p.tile = l.tile;
+    p.start = start;
+    p.slots = slots;
+    p.ranks = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + l.ranks);
+    p.counts = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + l.counts);
     CU_TRY(with_type(r->type, [&](auto zero) {
         using T = decltype(zero);
-        return with_layout(r->experts, [&](auto lpt, auto vpl) {
-            constexpr int L = decltype(lpt)::value, V = decltype(vpl)::value;
-            route_kernel<T, L, V><<<blocks_for(static_cast<int64_t>(tokens) * L, kRouteThreads),
-                                    kRouteThreads, 0, st>>>(p);
+        return with_layout(r->experts, [&](auto lpt, auto vpl, auto nt) {
+            constexpr int L = decltype(lpt)::value, V = decltype(vpl)::value, N = decltype(nt)::value;
+            route_kernel<T, L, V, N><<<l.tiles, N, 0, st>>>(p);
             return cudaGetLastError();
         });
     }), "route launch");
-    if (start) {
-        lists_kernel<<<r->experts + 1, 256, 0, st>>>(ids, tokens * r->k, r->experts, start, slots);
-        CU_TRY(cudaGetLastError(), "lists launch");
-    }
+    if (start && l.tiles > 1)
+        CU_TRY(launch_after(lists_kernel, dim3(l.tiles), kListThreads, 0, st, p), "lists launch");
     return ST_OK;
 }
 
@@ -619,10 +938,10 @@ extern "C" int mflat_cu_route_backward(const mflat_cu_router_t* r, const void* l
     p.ids = const_cast<int32_t*>(ids);
     CU_TRY(with_type(r->type, [&](auto zero) {
         using T = decltype(zero);
-        return with_layout(r->experts, [&](auto lpt, auto vpl) {
+        return with_layout(r->experts, [&](auto lpt, auto vpl, auto) {
             constexpr int L = decltype(lpt)::value, V = decltype(vpl)::value;
             route_backward_kernel<T, L, V>
-                <<<blocks_for(static_cast<int64_t>(tokens) * L, kRouteThreads), kRouteThreads, 0, st>>>(
+                <<<blocks_for(static_cast<int64_t>(tokens) * L, kGradThreads), kGradThreads, 0, st>>>(
                     p, grad_weights, static_cast<T*>(grad), grad_stride);
             return cudaGetLastError();
         });
