@@ -46,12 +46,6 @@ constexpr double kLn2 = 0.6931471805599453094;
 // kLow (the gap between the two is far below any sum's last digit).
 constexpr float kWild = 5e5f, kLow = -4e5f;
 
-__device__ __forceinline__ float exp2_fast(float t) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    return e;
-}
-
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;

@@ -12,7 +12,8 @@
 // among those of the same expert in its tile (in order: warps own adjacent choices
 // and count in histograms of their own) and leaves its count per expert; a second
 // kernel sums the counts of the tiles before and scatters.  Nothing depends on
-// the order in which blocks run.
+// the order in which blocks run.  Up to kClusterTokens tokens the tiles' blocks are one
+// cluster, which exchanges the counts in shared memory and scatters by itself.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -38,6 +39,7 @@ constexpr int kMaxExperts = 1024, kMaxRouteK = 32, kMaxGroups = 32;
 constexpr int kGradThreads = 256;
 constexpr int kCandMax = 64;        // candidates of a token that one warp ranks
 constexpr int kTiles = 148;         // one tile an SM
+constexpr int kClusterTiles = 8, kClusterTokens = 512;
 
 struct RouteParams {
     const void* logits;
@@ -50,26 +52,35 @@ struct RouteParams {
     const uint8_t* mask;
     int32_t* ids;
     float* weights;
+    int k_lanes;                // k rounded up to a power of two
     int lane_groups;            // lanes that share a group where that is a power of two, else 0
     // lists
     int tiles, tile;            // tokens per tile
+    int cluster;                // the tiles' blocks are one cluster
     uint16_t* ranks;            // workspace [tokens * k]: rank among the tile's choices of the expert
     uint16_t* counts;           // workspace [tiles][experts rounded up to 2]
     int32_t* start;
     int32_t* slots;
 };
 
-// Error bounds of an fp32 choice score and of a sum of two.  The scores are in
-// [0, 1] and formed with errors below 1e-6 (expf by exp2 of a rounded product:
-// relative 2^-22 + |x| 2^-24, which sigmoid and softmax damp by their own
-// value, a division of 2 ulp, and a sum of at most 1024 terms in a tree); adding
-// the bias rounds once more.  Twice that, for the two sides of a gap.
-__device__ __forceinline__ float tau_of(float c) { return 4e-6f + 3e-7f * fabsf(c); }
+// Bounds of the errors of the two fp32 scores on the sides of a gap.  sigmoid = 1 / (1 + e):
+// e is off by 2^-22 + |x| 2^-23 of itself, which reaches s times 1 - s (below 8e-8),
+// 1 + e rounds (6e-8), the division is off by 2 ulp (1.2e-7).  softmax = e / sum: relative
+// errors of e (3e-7 at distances that matter), of the sum (3e-7 and |x - m| 2^-23
+// weighted by the terms, at most ln 1024 + 1 on average: 1e-6; a chain of at most 31
+// additions a lane weighted likewise, 5 levels: 7e-7 for 8 experts a lane, 2.2e-6 for
+// 32) and of the division, all of a score of at most the row's largest.  Adding the
+// bias rounds once more, 6e-8 of the result.
+__device__ __forceinline__ float tau_base(bool softmax, float largest, int per_lane) {
+    return softmax ? 2.0f * (1.9e-6f + 6e-8f * per_lane) * largest + 2e-7f * largest : 5.4e-7f;
+}
+__device__ __forceinline__ float tau_of(float base, float c) { return base + 1.3e-7f * fabsf(c); }
 
 template <class S>
 __device__ __forceinline__ S exp_of(S v);
+constexpr float kLog2e = 1.4426950408889634f;
 template <>
-__device__ __forceinline__ float exp_of<float>(float v) { return __expf(v); }
+__device__ __forceinline__ float exp_of<float>(float v) { return exp2_fast(v * kLog2e); }
 template <>
 __device__ __forceinline__ double exp_of<double>(double v) { return exp(v); }
 
@@ -96,8 +107,14 @@ __device__ __forceinline__ S lane_sum(S v) {
 
 // Scores of the lane's experts, lane l of a token holding experts
 // [l * VPL, (l + 1) * VPL).  x: fp32 logits, -inf for "none".
+template <class S>
+__device__ __forceinline__ S inverse(S v) {
+    if constexpr (sizeof(S) == 4) return inverse_fast(v);
+    else return S(1) / v;
+}
 template <class S, int LPT, int VPL>
-__device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S (&s)[VPL]) {
+__device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S (&s)[VPL], S& largest) {
+    largest = S(1);
     if (softmax) {
         float m = neg_inf();
 #pragma unroll
@@ -111,12 +128,13 @@ __device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S
             sum += s[j];
         }
         sum = lane_sum<LPT>(sum);
-        const S inv = sum > S(0) ? S(1) / sum : S(0);
+        const S inv = sum > S(0) ? inverse(sum) : S(0);
+        largest = inv;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) s[j] *= inv;
     } else {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = S(1) / (S(1) + exp_of<S>(-S(x[j])));
+        for (int j = 0; j < VPL; ++j) s[j] = inverse(S(1) + exp_of<S>(-S(x[j])));
     }
 }
 
@@ -124,7 +142,7 @@ __device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S
 // gets the score of group g; tau the bound of the sums' errors.
 template <class S, int LPT, int VPL>
 __device__ __forceinline__ S group_scores(const RouteParams& p, int lane, const S (&c)[VPL],
-                                          const bool (&in)[VPL], float& tau) {
+                                          const bool (&in)[VPL], float base, float& tau) {
     const S none = S(neg_inf());
     const int size = p.experts / p.groups;
     S mine = none;
@@ -148,7 +166,7 @@ __device__ __forceinline__ S group_scores(const RouteParams& p, int lane, const 
         }
         const bool two = p.group_top == 2 && b != none;
         if (lane == g) mine = two ? a + b : a;
-        if (a != none) tau = fmaxf(tau, tau_of(float(a)) + (two ? tau_of(float(b)) : 0.0f));
+        if (a != none) tau = fmaxf(tau, tau_of(base, float(a)) + (two ? tau_of(base, float(b)) : 0.0f));
     }
     return mine;
 }
@@ -201,22 +219,28 @@ __device__ __forceinline__ void take_best(K (&key)[VPL], const float (&x)[VPL], 
 // the score.  Renormalised: scores over their sum, formed from exponents relative
 // to the largest chosen logit (sigmoid: to min(that, 0)), so that scores too
 // small for fp32 still have their quotient.
-template <int LPT>
 __device__ __forceinline__ float weight_of(const RouteParams& p, bool chosen, float x, float m,
                                            float sum) {
     float w = 0.0f;
     if (p.renormalise) {
+        // the choices are in the first lanes: exchanges over a power of two of them
         float top = chosen ? x : neg_inf();
-#pragma unroll
-        for (int o = LPT / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+        for (int o = p.k_lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
         if (chosen) {
-            if (p.softmax) w = x == top ? 1.0f : expf(x - top);
-            else w = x >= 0.0f ? 1.0f / (1.0f + expf(-x)) : expf(x - fminf(top, 0.0f)) / (1.0f + expf(x));
+            if (p.softmax) {
+                w = x == top ? 1.0f : expf(x - top);
+            } else if (top >= 0.0f) {
+                const float e = expf(-fabsf(x));
+                w = (x >= 0.0f ? 1.0f : e) * inverse_fast(1.0f + e);
+            } else {
+                w = expf(x - top) * inverse_fast(1.0f + expf(x));
+            }
         }
-        const float total = lane_sum<LPT>(w);
-        w = total > 0.0f ? w / total : 0.0f;
+        float total = w;
+        for (int o = p.k_lanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(kFullMask, total, o);
+        w = total > 0.0f ? w * inverse_fast(total) : 0.0f;
     } else if (chosen) {
-        w = p.softmax ? (x == m ? 1.0f : expf(x - m)) / sum : 1.0f / (1.0f + expf(-x));
+        w = p.softmax ? (x == m ? 1.0f : expf(x - m)) * inverse_fast(sum) : inverse_fast(1.0f + expf(-x));
     }
     return w * p.scale;
 }
@@ -259,7 +283,8 @@ __device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int la
     if (p.bias || (p.groups > 1 && p.group_top == 2)) {
         double c[VPL];
         bool in[VPL];
-        scores_of<double, LPT, VPL>(x, p.softmax, c);
+        double largest;
+        scores_of<double, LPT, VPL>(x, p.softmax, c, largest);
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             const int e = lane * VPL + j;
@@ -270,7 +295,7 @@ __device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int la
         if (p.groups > 1) {
             float unused;
             const unsigned kept = kept_groups<double, LPT>(
-                p, lane, group_scores<double, LPT, VPL>(p, lane, c, in, unused));
+                p, lane, group_scores<double, LPT, VPL>(p, lane, c, in, 0.0f, unused));
             const int size = p.experts / p.groups;
 #pragma unroll
             for (int j = 0; j < VPL; ++j)
@@ -286,7 +311,7 @@ __device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int la
         if (p.groups > 1) {
             float unused;
             const unsigned kept = kept_groups<float, LPT>(
-                p, lane, group_scores<float, LPT, VPL>(p, lane, x, in, unused));
+                p, lane, group_scores<float, LPT, VPL>(p, lane, x, in, 0.0f, unused));
             const int size = p.experts / p.groups;
 #pragma unroll
             for (int j = 0; j < VPL; ++j)
@@ -301,16 +326,16 @@ __device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int la
 // ties, which go to the lower group).  Where a group is 2^n lanes of a warp, their
 // top two meet in n exchanges, and each group is compared with all others: kept for
 // sure, dropped for sure, or in doubt.
-template <int LPT, int VPL>
+template <int LPT, int VPL, bool exact>
 __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, const float (&c)[VPL],
-                                              bool exact, float (&key)[VPL]) {
+                                              float base_tau, float (&key)[VPL]) {
     const float none = neg_inf();
     if (p.lane_groups == 0) {
         bool in[VPL];
         float tau;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) in[j] = key[j] > none;
-        const float mine = group_scores<float, LPT, VPL>(p, lane, c, in, tau);
+        const float mine = group_scores<float, LPT, VPL>(p, lane, c, in, base_tau, tau);
         const unsigned kept = kept_groups<float, LPT>(p, lane, mine);
         const int size = p.experts / p.groups;
         const bool here = lane < p.groups && ((kept >> lane) & 1u);
@@ -339,20 +364,26 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
     }
     const bool two = p.group_top == 2 && b > none;
     const float mine = two ? a + b : a;
-    float tau = a > none ? tau_of(a) + (two ? tau_of(b) : 0.0f) : 0.0f;
-#pragma unroll
-    for (int o = LPT / 2; o > 0; o >>= 1) tau = fmaxf(tau, __shfl_xor_sync(kFullMask, tau, o));
+    // all groups' largest; both terms are at least 0, so their bits order alike
+    float tau = a > none ? tau_of(base_tau, a) + (two ? tau_of(base_tau, b) : 0.0f) : 0.0f;
+    tau = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(tau)));
     if (exact) tau = 0.0f;
     const int base = (threadIdx.x & 31) - lane;
     const int group = lane / p.lane_groups;
-    int above = 0, near = 0;    // groups above for sure, and those not below for sure
+    // groups above for sure, and those not below for sure (itself among them)
+    int above = 0, near = 0;
+    const float high = mine + tau, low = mine - tau;
     for (int g = 0; g < p.groups; ++g) {
         const float v = __shfl_sync(kFullMask, mine, base + g * p.lane_groups);
-        const bool tie = v == mine && g < group;
-        above += (exact ? v > mine || tie : v > mine + tau) ? 1 : 0;
-        near += (g != group && (exact ? v > mine || tie : !(v < mine - tau))) ? 1 : 0;
+        if constexpr (exact) {
+            above += v > mine || (v == mine && g < group) ? 1 : 0;
+        } else {
+            above += v > high ? 1 : 0;
+            near += !(v < low) ? 1 : 0;
+        }
     }
-    const bool kept = near < p.groups_kept, dropped = above >= p.groups_kept || mine == none;
+    const bool kept = exact ? above < p.groups_kept : near <= p.groups_kept;
+    const bool dropped = above >= p.groups_kept || mine == none;
     if (!kept) {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) key[j] = none;
@@ -366,33 +397,80 @@ struct RouteScratch {
     float2 best[kMaxRouteK + 1];
 };
 
+// The choice scores of a token's n candidates in 64 bits, lane l those of candidates
+// l and l + 32.  The row is read again, so that the common path keeps its registers.
+template <class T>
+__device__ __noinline__ void refine(const RouteParams& p, const T* row, const RouteScratch& sh, int n,
+                                    double (&c)[2]) {
+    const int lane = threadIdx.x & 31;
+    double m = 0.0, sum = 1.0;
+    if (p.softmax) {
+        float mf = neg_inf();
+        for (int e = lane; e < p.experts; e += 32) mf = fmaxf(mf, to_float(row[e]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mf = fmaxf(mf, __shfl_xor_sync(kFullMask, mf, o));
+        m = mf;
+        sum = 0.0;
+        for (int e = lane; e < p.experts; e += 32) {
+            const float v = to_float(row[e]);
+            if (v > neg_inf()) sum += v == mf ? 1.0 : exp(static_cast<double>(v) - m);
+        }
+        sum = lane_sum<32>(sum);
+    }
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h;
+        c[h] = static_cast<double>(neg_inf());
+        if (i < n) {
+            const int e = __float_as_int(sh.cand[i].y);
+            const double v = to_float(row[e]);
+            const double s = p.softmax ? (v == m ? 1.0 : exp(v - m)) / sum : 1.0 / (1.0 + exp(-v));
+            c[h] = s + static_cast<double>(p.bias[e]);
+        }
+    }
+}
+
 // The k largest fp32 keys of a token that a whole warp holds (VPL > 1).  The k-th
 // largest lane maximum is a floor that few keys reach; those are ranked by counting.
-// Lane r gets the r-th expert, or -1.  Returns whether it has to be done exactly: with
-// `check` where neighbours are too close for fp32, and for more candidates than fit.
-template <int VPL>
-__device__ __forceinline__ bool take_best_warp(const float (&key)[VPL], int k, bool check,
+// Lane r gets the r-th expert, or -1.  With a bias, the floor is lower by tau, and
+// where neighbours in the selection are too close for fp32, its candidates are ranked
+// again by scores in 64 bits.  Returns whether there were more candidates than fit.
+template <class T, int VPL>
+__device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* row, const float (&key)[VPL],
+                                               float base_tau,
                                                RouteScratch& sh, int& id) {
-    const int lane = threadIdx.x & 31;
-    const int want = min(k + (check ? 1 : 0), 32);
+    const int lane = threadIdx.x & 31, k = p.k;
+    const bool check = p.bias != nullptr;
     float top = key[0];
 #pragma unroll
     for (int j = 1; j < VPL; ++j) top = fmaxf(top, key[j]);
-    float v = top;
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int o = size >> 1; o > 0; o >>= 1) {
-            const float w = __shfl_xor_sync(kFullMask, v, o);
-            const bool larger = ((lane & size) == 0) == ((lane & o) == 0);
-            v = larger ? fmaxf(v, w) : fminf(v, w);
+    float floor_v;
+    if (k <= 8) {
+        // k maxima, each with all its equals taken out: 3 instructions each
+        uint32_t v = choice_key(top), m = 0;
+        for (int r = 0; r < k; ++r) {
+            m = __reduce_max_sync(kFullMask, v);
+            v = v == m ? 0u : v;
         }
-    const float floor_v = __shfl_sync(kFullMask, v, want - 1);
+        floor_v = key_value(m);
+    } else {
+        float v = top;
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+            for (int o = size >> 1; o > 0; o >>= 1) {
+                const float w = __shfl_xor_sync(kFullMask, v, o);
+                const bool larger = ((lane & size) == 0) == ((lane & o) == 0);
+                v = larger ? fmaxf(v, w) : fminf(v, w);
+            }
+        floor_v = __shfl_sync(kFullMask, v, k - 1);
+    }
+    if (check) floor_v -= tau_of(base_tau, floor_v);
     const unsigned below = (1u << lane) - 1u;
     int n = 0;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        const bool in = key[j] >= floor_v && key[j] > neg_inf();
+        const bool in = !(key[j] < floor_v) && key[j] > neg_inf();
         const unsigned who = __ballot_sync(kFullMask, in);
         const int at = n + __popc(who & below);
         if (in && at < kCandMax) sh.cand[at] = make_float2(key[j], __int_as_float(lane * VPL + j));
@@ -404,6 +482,7 @@ __device__ __forceinline__ bool take_best_warp(const float (&key)[VPL], int k, b
         const float2 c = sh.cand[i];
         const int e = __float_as_int(c.y);
         int rank = 0;
+#pragma unroll 4
         for (int m = 0; m < n; ++m) {
             const float2 d = sh.cand[m];
             rank += d.x > c.x || (d.x == c.x && __float_as_int(d.y) < e) ? 1 : 0;
@@ -413,17 +492,32 @@ __device__ __forceinline__ bool take_best_warp(const float (&key)[VPL], int k, b
     __syncwarp();
     const float2 mine = lane < n && lane <= k ? sh.best[lane] : make_float2(neg_inf(), 0.0f);
     id = lane < k && lane < n ? __float_as_int(mine.y) : -1;
-    bool doubt = false;
     if (check) {
         // lane k holds the first that stays out (k = 32: look it up)
         float next = __shfl_down_sync(kFullMask, mine.x, 1);
         if (lane == 31) next = k == 32 && n > 32 ? sh.best[32].x : neg_inf();
-        doubt = lane < k && next > neg_inf() && !(mine.x - next > tau_of(mine.x));
-        // 32 lane maxima vouch for 32 candidates, not for the one after
-        doubt |= k == 32 && n <= 32;
+        const bool close = lane < k && next > neg_inf() && !(mine.x - next > tau_of(base_tau, mine.x));
+        if (__any_sync(kFullMask, close)) {
+            double c[2];
+            refine<T>(p, row, sh, n, c);
+            __syncwarp();
+            id = -1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int e = lane + 32 * h < n ? __float_as_int(sh.cand[lane + 32 * h].y) : 0;
+                int rank = 0;
+                for (int m = 0; m < n; ++m) {
+                    const double d = __shfl_sync(kFullMask, m < 32 ? c[0] : c[1], m & 31);
+                    rank += d > c[h] || (d == c[h] && __float_as_int(sh.cand[m].y) < e) ? 1 : 0;
+                }
+                if (lane + 32 * h < n && rank < k) sh.best[rank].y = __int_as_float(e);
+            }
+            __syncwarp();
+            if (lane < k && lane < n) id = __float_as_int(sh.best[lane].y);
+        }
     }
     __syncwarp();
-    return __any_sync(kFullMask, doubt);
+    return false;
 }
 
 // Exclusive sums of one value per thread's run over the block's values v[0, n) in
@@ -464,14 +558,14 @@ __device__ __forceinline__ void block_exclusive(int* v, int n, int* warp_sum) {
 }
 
 // One tile of tokens a block, LPT lanes per token, VPL experts per lane.  With lists,
-// then the ranks of the tile's choices and its counts; one tile alone goes all the way.
+// then the ranks of the tile's choices and its counts; a cluster goes all the way.
 template <class T, int LPT, int VPL, int NT>
 __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ RouteParams p) {
     constexpr int kWarps = NT / 32, kAtOnce = NT / LPT, kMost = LPT * VPL;
     __shared__ RouteScratch scratch[VPL > 1 ? kWarps : 1];
     const int lane = threadIdx.x % LPT, warp = threadIdx.x >> 5;
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
-    const int64_t t1 = min(t0 + p.tile, static_cast<int64_t>(p.tokens));
+    const int64_t t1 = max(t0, min(t0 + p.tile, static_cast<int64_t>(p.tokens)));
     const bool by_sums = p.bias || (p.groups > 1 && p.group_top == 2);
     float b[VPL];
 #pragma unroll
@@ -495,28 +589,32 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
             sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < VPL; ++j)
-                sum += x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : __expf(x[j] - m);
+                sum += x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : exp_of<float>(x[j] - m);
             sum = lane_sum<LPT>(sum);
         }
         bool doubt = false;
+        float base_tau = 0.0f;
         if (by_sums) {
-            float c[VPL];
-            scores_of<float, LPT, VPL>(x, p.softmax, c);
+            float c[VPL], largest;
+            scores_of<float, LPT, VPL>(x, p.softmax, c, largest);
+            base_tau = tau_base(p.softmax, largest, VPL);
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
                 c[j] += b[j];
-                key[j] = p.bias ? (x[j] > neg_inf() && c[j] > neg_inf() ? c[j] : neg_inf()) : x[j];
+                // (a bias of NaN makes a key that no comparison takes)
+                key[j] = !p.bias ? x[j] : x[j] > neg_inf() ? c[j] : neg_inf();
             }
-            if (p.groups > 1) doubt = choose_groups<LPT, VPL>(p, lane, c, false, key);
+            if (p.groups > 1) doubt = choose_groups<LPT, VPL, false>(p, lane, c, base_tau, key);
         } else {
 #pragma unroll
             for (int j = 0; j < VPL; ++j) key[j] = x[j];
-            if (p.groups > 1) choose_groups<LPT, VPL>(p, lane, x, true, key);
+            if (p.groups > 1) choose_groups<LPT, VPL, true>(p, lane, x, 0.0f, key);
         }
         int id = -1;
         float xid = neg_inf();
         if constexpr (VPL > 1) {
-            doubt |= take_best_warp<VPL>(key, p.k, p.bias != nullptr, scratch[warp], id);
+            doubt |= take_best_warp<T, VPL>(p, static_cast<const T*>(p.logits) + t * p.stride, key,
+                                            base_tau, scratch[warp], id);
         } else {
             // one expert a lane: its rank by counting
             const int base = (threadIdx.x & 31) - lane;
@@ -530,7 +628,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
                 next = !before && e != lane ? fmaxf(next, v) : next;
             }
             if (!(key[0] > neg_inf())) rank = LPT;
-            if (p.bias && rank < p.k && next > neg_inf()) doubt |= !(key[0] - next > tau_of(key[0]));
+            if (p.bias && rank < p.k && next > neg_inf()) doubt |= !(key[0] - next > tau_of(base_tau, key[0]));
             for (int r = 0; r < p.k; ++r) {
                 const unsigned who = __ballot_sync(kFullMask, rank == r) >> base;
                 const unsigned own = LPT == 32 ? who : who & ((1u << (LPT & 31)) - 1u);
@@ -542,7 +640,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
         } else if (id >= 0) {
             xid = to_float(static_cast<const T*>(p.logits)[t * p.stride + id]);
         }
-        const float w = weight_of<LPT>(p, id >= 0, xid, m, sum);
+        const float w = weight_of(p, id >= 0, xid, m, sum);
         if (t < t1 && lane < p.k) {
             p.ids[t * p.k + lane] = id;
             p.weights[t * p.k + lane] = w;
@@ -552,7 +650,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
 
     // ranks: warps own adjacent runs of the tile's choices
     __shared__ uint16_t hist[kWarps][kMost];
-    __shared__ int total[kMost + 1];
+    __shared__ int total[kMost + 1], before[kMost];
     __shared__ int warp_sum[32];
     const int full_lane = threadIdx.x & 31;
     for (int i = threadIdx.x; i < kWarps * kMost / 2; i += NT) reinterpret_cast<uint32_t*>(&hist[0][0])[i] = 0;
@@ -561,48 +659,84 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
     const int64_t e0 = t0 * p.k, n = (t1 - t0) * p.k;
     const int64_t run = (n + kWarps * 32 - 1) / (kWarps * 32) * 32;
     const int64_t r0 = e0 + warp * run, r1 = min(r0 + run, e0 + n);
+    // a run of one step (a tile of up to 32 choices a warp) stays in registers
+    const bool one = run == 32;
+    int own_id = -1, own_rank = 0;
     for (int64_t i0 = r0; i0 < r1; i0 += 32) {
         const int64_t i = i0 + full_lane;
         const int id = i < r1 ? p.ids[i] : -1;
         const unsigned peers = __match_any_sync(kFullMask, id);
         const int rank = __popc(peers & ((1u << full_lane) - 1u));
-        int before = 0;
+        int seen = 0;
         if (id >= 0 && rank == 0) {
-            before = hist[warp][id];
-            hist[warp][id] = static_cast<uint16_t>(before + __popc(peers));
+            seen = hist[warp][id];
+            hist[warp][id] = static_cast<uint16_t>(seen + __popc(peers));
         }
-        before = __shfl_sync(kFullMask, before, __ffs(peers) - 1);
-        if (id >= 0) p.ranks[i] = static_cast<uint16_t>(before + rank);
+        seen = __shfl_sync(kFullMask, seen, __ffs(peers) - 1);
+        own_id = id;
+        own_rank = seen + rank;
+        if (!one && id >= 0) p.ranks[i] = static_cast<uint16_t>(own_rank);
         __syncwarp();
     }
     __syncthreads();
     for (int e = threadIdx.x; e < p.experts; e += NT) {
         int s = 0;
-#pragma unroll 8
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const int c = hist[w][e];
             hist[w][e] = static_cast<uint16_t>(s);
             s += c;
         }
         total[e] = s;
-        if (p.tiles > 1) p.counts[static_cast<int64_t>(blockIdx.x) * ((p.experts + 1) & ~1) + e] = static_cast<uint16_t>(s);
+        if (!p.cluster) p.counts[static_cast<int64_t>(blockIdx.x) * ((p.experts + 1) & ~1) + e] = static_cast<uint16_t>(s);
     }
-    if (p.tiles > 1) {
-        __syncthreads();
+    // fn(choice, expert, rank in the tile) for the thread's choices
+    auto each = [&](auto&& fn) {
+        if (one) {
+            if (own_id >= 0) fn(r0 + full_lane, own_id, own_rank + hist[warp][own_id]);
+            return;
+        }
         for (int64_t i = r0 + full_lane; i < r1; i += 32) {
             const int id = p.ids[i];
-            if (id >= 0) p.ranks[i] = static_cast<uint16_t>(p.ranks[i] + hist[warp][id]);
+            if (id >= 0) fn(i, id, p.ranks[i] + hist[warp][id]);
         }
+    };
+    if (!p.cluster) {
+        __syncthreads();
+        each([&](int64_t i, int, int rank) { p.ranks[i] = static_cast<uint16_t>(rank); });
         return;
+    }
+    cluster_sync();             // every block's counts are in its total[]
+    const uint32_t me = cluster_rank();
+    int sums[(kMost + NT - 1) / NT];
+#pragma unroll
+    for (int j = 0; j < (kMost + NT - 1) / NT; ++j) {
+        const int e = j * NT + threadIdx.x;
+        int all = 0, ahead = 0;
+        if (e < p.experts) {
+#pragma unroll
+            for (uint32_t r = 0; r < kClusterTiles; ++r) {
+                int c;
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(cluster_addr(&total[e], r)) : "memory");
+                all += c;
+                ahead += r < me ? c : 0;
+            }
+            before[e] = ahead;
+        }
+        sums[j] = all;
+    }
+    cluster_sync();             // and read by all: total[] is free again
+#pragma unroll
+    for (int j = 0; j < (kMost + NT - 1) / NT; ++j) {
+        const int e = j * NT + threadIdx.x;
+        if (e < p.experts) total[e] = sums[j];
     }
     if (threadIdx.x == 0) total[p.experts] = 0;
     __syncthreads();
     block_exclusive<NT>(total, p.experts + 1, warp_sum);
-    for (int e = threadIdx.x; e <= p.experts; e += NT) p.start[e] = total[e];
-    for (int64_t i = r0 + full_lane; i < r1; i += 32) {
-        const int id = p.ids[i];
-        if (id >= 0) p.slots[total[id] + hist[warp][id] + p.ranks[i]] = static_cast<int32_t>(i);
-    }
+    if (me == 0)
+        for (int e = threadIdx.x; e <= p.experts; e += NT) p.start[e] = total[e];
+    each([&](int64_t i, int id, int rank) { p.slots[total[id] + before[id] + rank] = static_cast<int32_t>(i); });
 }
 
 // The lists of many tiles: where this tile's choices of each expert begin, then the
@@ -695,7 +829,7 @@ __global__ void __launch_bounds__(kGradThreads)
         sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-            d[j] = x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : __expf(x[j] - m);
+            d[j] = x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : exp_of<float>(x[j] - m);
             sum += d[j];
         }
         sum = lane_sum<LPT>(sum);
@@ -705,7 +839,7 @@ __global__ void __launch_bounds__(kGradThreads)
     }
     RouteParams q = p;
     q.scale = 1.0f;
-    const float w = weight_of<LPT>(q, chosen, xid, m, sum);
+    const float w = weight_of(q, chosen, xid, m, sum);
     const float dot = (p.softmax || p.renormalise) ? lane_sum<LPT>(g * w) : 0.0f;
     if (whole) {
         const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
@@ -809,19 +943,26 @@ int check_router(const mflat_cu_router_t* r, int tokens) {
     return ST_OK;
 }
 
-// Tiles of the lists: one to an SM, no more tokens in one than 16-bit counts hold; up
-// to kOneTile tokens a single tile, whose block needs no second kernel.
-constexpr int kOneTile = 64;
+// Tiles: one to an SM, no more tokens in one than 16-bit counts hold; up to
+// kClusterTokens tokens (with lists), one to a block of a cluster.
 struct RoutePlan {
+    bool cluster;
     int tiles, tile;
     size_t ranks, counts, end;
 };
 RoutePlan route_plan(const mflat_cu_router_t* r, int tokens) {
     RoutePlan l{};
-    l.tiles = tokens <= kOneTile ? 1 : kTiles;
+    // a cluster's block keeps its choices in registers, one a thread
+    const int threads = r->experts <= 256 ? 1024 : r->experts <= 512 ? 512 : 256;
+    l.tile = (tokens + kClusterTiles - 1) / kClusterTiles;
+    if (tokens <= kClusterTokens && l.tile * r->k <= threads) {
+        l.cluster = true;
+        l.tiles = kClusterTiles;
+        return l;
+    }
+    l.tiles = kTiles;
     l.tile = (tokens + l.tiles - 1) / l.tiles;
     if (l.tile > 65535) l.tile = 65535;
-    if (tokens > kOneTile && l.tile < 32) l.tile = 32;
     l.tiles = (tokens + l.tile - 1) / l.tile;
     auto round256 = [](size_t n) { return (n + 255) & ~size_t(255); };
     l.ranks = 0;
@@ -848,6 +989,8 @@ int fill_params(const mflat_cu_router_t* r, const void* logits, int64_t& stride,
     p.group_top = r->group_top;
     p.scale = r->scale;
     p.vec = packed_rows(logits, stride, r->experts, type_bytes(r->type));
+    p.k_lanes = 1;
+    while (p.k_lanes < r->k) p.k_lanes *= 2;
     int vpl = 1;
     while (vpl * 32 < r->experts) vpl *= 2;
     const int size = r->experts / r->groups;
@@ -897,6 +1040,11 @@ extern "C" int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, in
     const RoutePlan l = route_plan(r, tokens);
     p.tiles = l.tiles;
     p.tile = l.tile;
+    if (!start && l.cluster) {      // no lists: over all SMs
+        p.tile = (tokens + kTiles - 1) / kTiles;
+        p.tiles = (tokens + p.tile - 1) / p.tile;
+    }
+    p.cluster = start && l.cluster;
     p.start = start;
     p.slots = slots;
     p.ranks = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + l.ranks);
@@ -905,11 +1053,12 @@ extern "C" int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, in
         using T = decltype(zero);
         return with_layout(r->experts, [&](auto lpt, auto vpl, auto nt) {
             constexpr int L = decltype(lpt)::value, V = decltype(vpl)::value, N = decltype(nt)::value;
-            route_kernel<T, L, V, N><<<l.tiles, N, 0, st>>>(p);
+            if (p.cluster) return launch_cluster(route_kernel<T, L, V, N>, p.tiles, N, st, p);
+            route_kernel<T, L, V, N><<<p.tiles, N, 0, st>>>(p);
             return cudaGetLastError();
         });
     }), "route launch");
-    if (start && l.tiles > 1)
+    if (start && !l.cluster)
         CU_TRY(launch_after(lists_kernel, dim3(l.tiles), kListThreads, 0, st, p), "lists launch");
     return ST_OK;
 }

@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "index_impl.cuh"
+#include "ptx.cuh"
 
 namespace mflat_cu {
 
@@ -33,6 +34,18 @@ template <class T, int N>
 struct alignas(N * sizeof(T)) Pack {
     T v[N];
 };
+
+// 2^t and 1/v by the special function unit, 2^-22 and 2 ulp off, subnormals flushed.
+__device__ __forceinline__ float exp2_fast(float t) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    return e;
+}
+__device__ __forceinline__ float inverse_fast(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 
 // Keys whose order is the value's, for selection by integer comparison.
 // Equal values (-0 and +0 among them) get equal keys; 0 is left for "no
@@ -76,6 +89,24 @@ cudaError_t launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+// All blocks of the grid as one cluster.
+template <class... P, class... A>
+cudaError_t launch_cluster(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t st,
+                           A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = blocks;
+    at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
