@@ -7,6 +7,10 @@
 // entries below m ("holes") take the kept entries at and behind m ("tails") in
 // order: sources lie behind m and targets below it, so rows move in place in any
 // order.
+//
+// One kernel does it all: a cluster of 1 to 8 blocks owns a (sequence, head), keeps
+// its sums and keys in shared memory and exchanges histograms and counts there.
+// The three kernels behind it are for caches longer than eight blocks hold.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -18,6 +22,9 @@
 namespace mflat_cu {
 namespace {
 
+constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictSlots = 24576;      // slots a block holds, 8 bytes each
+constexpr int kEvictCluster = 8;
 constexpr int kAccThreads = 256;
 constexpr int kKeepThreads = 512, kKeepWarps = kKeepThreads / 32;
 
@@ -26,6 +33,7 @@ struct CacheParams {
     int64_t wb, wh, wq;
     int64_t kb, kh, ks, vb, vh, vs;     // bytes
     int64_t key_vecs, value_vecs;
+    int rows_vec;                       // bytes of a vector of the rows: 16, 4 or 1 (0: no rows)
     const void* weights;
     const int32_t* rows;
     const int32_t* lens;
@@ -37,14 +45,329 @@ struct CacheParams {
     int32_t* out_lens;
     char* keys;
     char* values;
-    float* sums;                        // workspace [b][h][capacity]: acc'
-    int32_t* holes;                     // workspace [b][h][capacity]
-    int32_t* tails;
-    int32_t* moves;                     // workspace [b][h]
+    int vec_w, vec_a;                   // weights, and acc and pos, can be read by fours
+    int range;                          // slots of a block of evict_kernel
+    int half;                           // most moves of a head: capacity / 2
+    float* sums;                        // long caches [b][h][capacity]: acc'
+    int32_t* holes;                     // workspace [b][h][half]
+    int32_t* tails;                     // workspace [b][h][half]: slot,
+    float* tail_acc;                    // acc' and
+    int32_t* tail_pos;                  // position
+    int32_t* moves;                     // long caches [b][h]
 };
 
 __device__ __forceinline__ int entries_of(const CacheParams& p, int b) {
     return min(max(p.lens[b], 0), p.capacity);
+}
+
+// The rows of a (sequence, head): keys then values, as one list of vectors.
+struct RowsOf {
+    char *keys, *values;
+    int64_t key_stride, value_stride, key_vecs, value_vecs;
+};
+
+// Moves first, first + stride, ... of n, a warp each, four at a time: their rows'
+// vectors are all read before the first is written.
+template <class V>
+__device__ __forceinline__ void move_rows(const RowsOf& p, const int32_t* holes, const int32_t* tails,
+                                          int first, int stride, int n) {
+    const int lane = threadIdx.x & 31;
+    for (int i0 = first; i0 < n; i0 += 4 * stride) {
+        int from[4], to[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(i0 + u * stride, n - 1);
+            from[u] = tails[i];
+            to[u] = holes[i];
+        }
+        for (int64_t c = lane; c < p.key_vecs + p.value_vecs; c += 32) {
+            const bool key = c < p.key_vecs;
+            char* base = (key ? p.keys : p.values) + (key ? c : c - p.key_vecs) * static_cast<int64_t>(sizeof(V));
+            const int64_t slot = key ? p.key_stride : p.value_stride;
+            V v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const V*>(base + from[u] * slot);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * stride < n) *reinterpret_cast<V*>(base + to[u] * slot) = v[u];
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t slot_key(const CacheParams& p, float acc, int pos, int64_t since) {
+    if (pos < p.sink || pos >= since) return 0xffffffffu;
+    return acc == neg_inf() ? 1u : choice_key(acc);     // NaN: 0
+}
+
+// Exclusive sum over the block's threads in order, and the block's total.
+__device__ __forceinline__ int scan_block(int v, int* warp_sum, int& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFullMask, incl, o);
+        if (lane >= o) incl += u;
+    }
+    __syncthreads();                // warp_sum is free
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kEvictWarps; ++w) {
+        const int c = warp_sum[w];
+        before += w < warp ? c : 0;
+        total += c;
+    }
+    return before + incl - v;
+}
+
+__device__ __forceinline__ int cluster_load(const int* p, uint32_t rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, rank)) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ int4 cluster_load4(const int* p, uint32_t rank) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(cluster_addr(p, rank))
+                 : "memory");
+    return v;
+}
+
+// Barrier over the blocks of a (sequence, head), for shared and global memory.
+__device__ __forceinline__ void sync_blocks(uint32_t blocks) {
+    if (blocks == 1) __syncthreads();
+    else cluster_sync();
+}
+
+constexpr int kRowsAtOnce = 8;
+
+// s[i] += the weights of slots j + i over the group's heads and `rows` query rows, in
+// 64 bits, kRowsAtOnce rows in flight.
+template <class T>
+__device__ __forceinline__ void add_rows(const T* w, int64_t wh, int64_t wq, int group, int rows, bool vec,
+                                         int most, double (&s)[4]) {
+    int g = 0, r = 0;
+    while (g < group) {
+        if (vec) {
+            Pack<T, 4> v[kRowsAtOnce];
+#pragma unroll
+            for (int u = 0; u < kRowsAtOnce; ++u) {
+                if (g < group) v[u] = *reinterpret_cast<const Pack<T, 4>*>(w + g * wh + r * wq);
+                else v[u] = Pack<T, 4>{};
+                if (++r == rows) {
+                    r = 0;
+                    ++g;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kRowsAtOnce; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] += static_cast<double>(to_float(v[u].v[i]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < most) s[i] += static_cast<double>(to_float(w[g * wh + r * wq + i]));
+            if (++r == rows) {
+                r = 0;
+                ++g;
+            }
+        }
+    }
+}
+
+// A (sequence, head): blockIdx.y; its blocks' ranges of slots: blockIdx.x, one cluster.
+// A thread adds up four adjacent slots at a time (the group's rows eight in flight),
+// then the m-th key is found by three digits of 11, 11 and 10 bits: histograms in
+// shared memory, summed over the cluster by every block.  Behind that a thread owns
+// a run of adjacent slots, so that one scan over the threads orders all of them.
+template <class T>
+__global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CacheParams p) {
+    extern __shared__ uint32_t dyn[];
+    __shared__ __align__(16) int hist[2][2048];
+    __shared__ int warp_sum[kEvictWarps];
+    __shared__ uint32_t sh_prefix;
+    __shared__ int sh_left, sh_ties, sh_moves;
+    uint32_t* keys = dyn;
+    float* sums = reinterpret_cast<float*>(dyn + p.range);
+    const int64_t bh = blockIdx.y;
+    const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh % p.heads);
+    const uint32_t me = blockIdx.x, blocks = gridDim.x;
+    const int n = entries_of(p, b), m = min(n, p.budget);
+    const int lo = static_cast<int>(me) * p.range;
+    const int mine = max(0, min(p.range, n - lo));      // live slots of this block
+    const float* acc = p.acc + bh * p.capacity + lo;
+    const int32_t* pos = p.pos + bh * p.capacity + lo;
+    float* out_acc = p.out_acc + bh * p.capacity;
+    int32_t* out_pos = p.out_pos + bh * p.capacity;
+    if (threadIdx.x == 0 && me == 0 && h == 0) p.out_lens[b] = m;
+    const bool over = n > p.budget;
+    const int64_t since = static_cast<int64_t>(p.seen[b]) - p.recent;
+
+    const int rows = !p.weights ? 0 : p.rows ? min(max(p.rows[b], 0), p.queries) : p.queries;
+    const T* weights = static_cast<const T*>(p.weights) + b * p.wb + static_cast<int64_t>(h) * p.group * p.wh + lo;
+    for (int j = threadIdx.x * 4; j < mine; j += kEvictThreads * 4) {
+        const int most = min(4, mine - j);
+        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        int q[4] = {0, 0, 0, 0};
+        if (p.vec_a && most == 4) {
+            const Pack<float, 4> va = *reinterpret_cast<const Pack<float, 4>*>(acc + j);
+            const Pack<int, 4> vq = *reinterpret_cast<const Pack<int, 4>*>(pos + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = va.v[i];
+                q[i] = vq.v[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < most) {
+                    a[i] = acc[j + i];
+                    q[i] = pos[j + i];
+                }
+        }
+        if (rows > 0) {
+            double s[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = a[i];
+            add_rows(weights + j, p.wh, p.wq, p.group, rows, p.vec_w && most == 4, most, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = static_cast<float>(s[i]);
+        }
+        if (over) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < most) {
+                    sums[j + i] = a[i];
+                    keys[j + i] = slot_key(p, a[i], q[i], since);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < most) {
+                    out_acc[lo + j + i] = a[i];
+                    out_pos[lo + j + i] = q[i];
+                }
+        }
+    }
+    if (!over) return;
+
+    if (threadIdx.x == 0) { sh_prefix = 0; sh_left = m; }
+    for (int i = threadIdx.x; i < 2048; i += kEvictThreads) hist[0][i] = 0;
+    __syncthreads();
+    uint32_t mask = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        const uint32_t prefix = sh_prefix, digits = (1u << bits) - 1u;
+        for (int j = threadIdx.x; j < mine; j += kEvictThreads) {
+            const uint32_t key = keys[j];
+            if ((key & mask) == prefix) atomicAdd(&hist[pass & 1][(key >> shift) & digits], 1);
+        }
+        sync_blocks(blocks);
+        // four digits a thread, from the top down
+        const int d0 = 2044 - static_cast<int>(threadIdx.x) * 4;
+        int4 c = *reinterpret_cast<const int4*>(&hist[pass & 1][d0]);
+        if (blocks > 1) {
+            c = make_int4(0, 0, 0, 0);
+#pragma unroll
+            for (uint32_t r = 0; r < kEvictCluster; ++r)
+                if (r < blocks) {
+                    const int4 o = cluster_load4(&hist[pass & 1][d0], r);
+                    c.x += o.x;
+                    c.y += o.y;
+                    c.z += o.z;
+                    c.w += o.w;
+                }
+        }
+        const int count[4] = {c.w, c.z, c.y, c.x}, sum = c.x + c.y + c.z + c.w;
+        // (read by the other blocks before this pass's cluster barrier)
+        if (pass < 2)
+            for (int i = threadIdx.x; i < 2048; i += kEvictThreads) hist[(pass + 1) & 1][i] = 0;
+        const int left = sh_left;
+        int total;
+        int above = scan_block(sum, warp_sum, total);       // its barriers: left is read
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (above < left && left <= above + count[i]) {
+                sh_prefix = prefix | (static_cast<uint32_t>(2047 - (threadIdx.x * 4 + i)) << shift);
+                sh_left = left - above;
+            }
+            above += count[i];
+        }
+        mask |= digits << shift;
+        __syncthreads();
+    }
+    const uint32_t cut = sh_prefix;
+    const int ties = sh_left;           // entries at the cut that stay, the lowest slots
+
+    // runs of an odd length: threads read different banks
+    const int run = ((mine + kEvictThreads - 1) / kEvictThreads) | 1;
+    const int j0 = min(mine, static_cast<int>(threadIdx.x) * run), j1 = min(mine, j0 + run);
+    int equal = 0, total;
+    for (int j = j0; j < j1; ++j) equal += keys[j] == cut ? 1 : 0;
+    int tie = scan_block(equal, warp_sum, total);
+    if (threadIdx.x == 0) sh_ties = total;
+    sync_blocks(blocks);
+    for (uint32_t r = 0; r < me; ++r) tie += cluster_load(&sh_ties, r);
+    const int tie0 = tie;
+    int moved = 0;                      // holes in the upper half word, tails in the lower
+    for (int j = j0; j < j1; ++j) {
+        const uint32_t key = keys[j];
+        const bool keep = key > cut || (key == cut && tie++ < ties);
+        if (lo + j < m ? !keep : keep) moved += lo + j < m ? 1 << 16 : 1;
+    }
+    const int rank = scan_block(moved, warp_sum, total);
+    if (threadIdx.x == 0) sh_moves = total;
+    sync_blocks(blocks);
+    int hole = rank >> 16, tail = rank & 0xffff, moves = 0;
+    for (uint32_t r = 0; r < blocks; ++r) {
+        const int c = cluster_load(&sh_moves, r);
+        hole += r < me ? c >> 16 : 0;
+        tail += r < me ? c & 0xffff : 0;
+        moves += c >> 16;
+    }
+    int32_t* holes = p.holes + bh * p.half;
+    int32_t* tails = p.tails + bh * p.half;
+    float* tail_acc = p.tail_acc + bh * p.half;
+    int32_t* tail_pos = p.tail_pos + bh * p.half;
+    tie = tie0;
+    for (int j = j0; j < j1; ++j) {
+        const uint32_t key = keys[j];
+        const bool keep = key > cut || (key == cut && tie++ < ties);
+        keys[j] = keep ? 1u : 0u;
+        if (lo + j < m) {
+            if (!keep) holes[hole++] = lo + j;
+        } else if (keep) {
+            tails[tail] = lo + j;
+            tail_acc[tail] = sums[j];
+            tail_pos[tail++] = pos[j];
+        }
+    }
+    sync_blocks(blocks);                // the lists are complete and in every block's sight
+    for (int j = threadIdx.x; j < mine && lo + j < m; j += kEvictThreads)
+        if (keys[j]) {
+            out_acc[lo + j] = sums[j];
+            if (p.out_pos != p.pos) out_pos[lo + j] = pos[j];
+        }
+    const int at = static_cast<int>(me) * kEvictThreads + threadIdx.x, step = static_cast<int>(blocks) * kEvictThreads;
+    for (int i = at; i < moves; i += step) {
+        const int to = holes[i];
+        out_acc[to] = tail_acc[i];
+        out_pos[to] = tail_pos[i];
+    }
+    // rows: a warp per move, keys and values
+    if (!p.rows_vec) return;
+    char* k = p.keys ? p.keys + b * p.kb + h * p.kh : nullptr;
+    char* v = p.values ? p.values + b * p.vb + h * p.vh : nullptr;
+    const RowsOf rows_of{k, v, p.ks, p.vs, p.key_vecs, p.value_vecs};
+    const int first = at >> 5, stride = step >> 5;
+    if (p.rows_vec == 16) move_rows<uint4>(rows_of, holes, tails, first, stride, moves);
+    else if (p.rows_vec == 4) move_rows<uint32_t>(rows_of, holes, tails, first, stride, moves);
+    else move_rows<uint8_t>(rows_of, holes, tails, first, stride, moves);
 }
 
 template <class T>
@@ -88,12 +411,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const CacheParams p)
         return;
     }
     const int64_t since = static_cast<int64_t>(p.seen[b]) - p.recent;
-    auto key_at = [&](int j) {
-        const int q = pos[j];
-        if (q < p.sink || q >= since) return 0xffffffffu;
-        const float a = sums[j];
-        return a == neg_inf() ? 1u : choice_key(a);
-    };
+    auto key_at = [&](int j) { return slot_key(p, sums[j], pos[j], since); };
     // the m-th largest key, 8 bits at a time
     if (threadIdx.x == 0) { sh_prefix = 0; sh_left = m; }
     uint32_t mask = 0;
@@ -117,8 +435,8 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const CacheParams p)
     }
     const uint32_t cut = sh_prefix;
     const int ties = sh_left;           // entries at the cut that stay
-    int32_t* holes = p.holes + bh * p.capacity;
-    int32_t* tails = p.tails + bh * p.capacity;
+    int32_t* holes = p.holes + bh * p.half;
+    int32_t* tails = p.tails + bh * p.half;
     int n_tie = 0, n_hole = 0, n_tail = 0;
     for (int j0 = 0; j0 < n; j0 += kKeepThreads) {
         const int j = j0 + threadIdx.x;
@@ -167,39 +485,44 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const CacheParams p)
     if (threadIdx.x == 0) p.moves[bh] = n_hole;
 }
 
-// Rows of keys (blockIdx.z 0) and values (1), a warp per move.
-template <class V>
 __global__ void __launch_bounds__(256) move_kernel(const CacheParams p) {
     const int64_t bh = blockIdx.y;
     const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh % p.heads);
-    char* base = blockIdx.z == 0 ? p.keys : p.values;
-    if (!base) return;
-    base += blockIdx.z == 0 ? b * p.kb + h * p.kh : b * p.vb + h * p.vh;
-    const int64_t slot = blockIdx.z == 0 ? p.ks : p.vs;
-    const int64_t vecs = blockIdx.z == 0 ? p.key_vecs : p.value_vecs;
-    const int n = p.moves[bh];
-    const int32_t* holes = p.holes + bh * p.capacity;
-    const int32_t* tails = p.tails + bh * p.capacity;
-    for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
-        const V* from = reinterpret_cast<const V*>(base + tails[i] * slot);
-        V* to = reinterpret_cast<V*>(base + holes[i] * slot);
-        for (int64_t v = threadIdx.x & 31; v < vecs; v += 32) to[v] = from[v];
-    }
+    const RowsOf rows_of{p.keys ? p.keys + b * p.kb + h * p.kh : nullptr,
+                         p.values ? p.values + b * p.vb + h * p.vh : nullptr, p.ks, p.vs, p.key_vecs, p.value_vecs};
+    const int32_t *holes = p.holes + bh * p.half, *tails = p.tails + bh * p.half;
+    const int n = p.moves[bh], first = blockIdx.x * 8 + (threadIdx.x >> 5), stride = gridDim.x * 8;
+    if (p.rows_vec == 16) move_rows<uint4>(rows_of, holes, tails, first, stride, n);
+    else if (p.rows_vec == 4) move_rows<uint32_t>(rows_of, holes, tails, first, stride, n);
+    else move_rows<uint8_t>(rows_of, holes, tails, first, stride, n);
 }
 
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Blocks of a cluster: as few as hold the slots, but enough to fill the machine with
+// ranges of at least 1024 slots.  0: too long for eight.
+int cluster_of(const mflat_cu_cache_t* c, int batch) {
+    const int64_t bh = static_cast<int64_t>(batch) * c->heads;
+    int n = 1;
+    auto range = [&] { return c->capacity / n + (c->capacity % n ? 1 : 0); };
+    while (n < kEvictCluster && (range() > kEvictSlots || (bh * n < 148 && range() >= 2048))) n *= 2;
+    return range() <= kEvictSlots ? n : 0;
+}
+
 struct CacheLayout {
-    size_t sums, holes, tails, moves, end;
+    size_t holes, tails, tail_acc, tail_pos, sums, moves, end;
 };
 CacheLayout cache_layout(const mflat_cu_cache_t* c, int batch) {
-    const size_t bh = static_cast<size_t>(batch) * c->heads, n = bh * c->capacity;
+    const size_t bh = static_cast<size_t>(batch) * c->heads, half = bh * (c->capacity / 2);
     CacheLayout l;
-    l.sums = 0;
-    l.holes = l.sums + round256(n * 4);
-    l.tails = l.holes + round256(n * 4);
-    l.moves = l.tails + round256(n * 4);
-    l.end = l.moves + round256(bh * 4);
+    l.holes = 0;
+    l.tails = l.holes + round256(half * 4);
+    l.tail_acc = l.tails + round256(half * 4);
+    l.tail_pos = l.tail_acc + round256(half * 4);
+    l.sums = l.tail_pos + round256(half * 4);
+    const bool is_long = cluster_of(c, batch) == 0;
+    l.moves = l.sums + (is_long ? round256(bh * c->capacity * 4) : 0);
+    l.end = l.moves + (is_long ? round256(bh * 4) : 0);
     return l;
 }
 
@@ -220,6 +543,27 @@ int check_cache(const mflat_cu_cache_t* c, int batch) {
         return fail(ST_BAD_ARG, msg);
     }
     return ST_OK;
+}
+
+// blockIdx.x runs over the cluster, blockIdx.y over the heads.
+template <class K>
+cudaError_t launch_evict(K kernel, int blocks, unsigned bh, size_t smem, cudaStream_t st, const CacheParams& p) {
+    // always the same bound: calls from several threads may set it at once
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSlots * 8);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks), bh);
+    cfg.blockDim = dim3(kEvictThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = static_cast<unsigned>(blocks);
+    at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 // Dense strides where all are 0; false where two rows could overlap.
@@ -283,7 +627,7 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
     if (batch == 0) return ST_OK;
     if (out_lens == lens) return fail(ST_BAD_ARG, "out_lens must not be lens");
     const CacheLayout l = cache_layout(c, batch);
-    if (!ws || ws_bytes < l.end || !aligned_to(ws, 256))
+    if (l.end > 0 && (!ws || ws_bytes < l.end || !aligned_to(ws, 256)))
         return fail(ST_BAD_ARG, "workspace missing, too small or not 256-byte aligned");
     rc = operator_device(device, &device);
     if (rc != ST_OK) return rc;
@@ -305,7 +649,27 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
     p.holes = reinterpret_cast<int32_t*>(w + l.holes);
     p.tails = reinterpret_cast<int32_t*>(w + l.tails);
     p.moves = reinterpret_cast<int32_t*>(w + l.moves);
+    p.tail_acc = reinterpret_cast<float*>(w + l.tail_acc);
+    p.tail_pos = reinterpret_cast<int32_t*>(w + l.tail_pos);
+    p.half = c->capacity / 2;
+    p.vec_w = ((p.wb | p.wh | p.wq) & 3) == 0 && aligned_to(weights, 4 * type_bytes(c->type));
+    p.vec_a = (c->capacity & 3) == 0 && aligned_to(acc, 16) && aligned_to(pos, 16);
+    int64_t bits = 0;
+    if (p.keys) bits |= c->key_bytes | p.kb | p.kh | p.ks | static_cast<int64_t>(reinterpret_cast<uintptr_t>(keys) & 15);
+    if (p.values) bits |= c->value_bytes | p.vb | p.vh | p.vs | static_cast<int64_t>(reinterpret_cast<uintptr_t>(values) & 15);
+    const int vec = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+    p.rows_vec = p.keys || p.values ? vec : 0;
+    p.key_vecs = p.keys ? c->key_bytes / vec : 0;
+    p.value_vecs = p.values ? c->value_bytes / vec : 0;
     const unsigned bh = static_cast<unsigned>(batch * c->heads);
+    const int blocks = cluster_of(c, batch);
+    if (blocks > 0) {
+        p.range = (c->capacity / blocks + (c->capacity % blocks ? 1 : 0) + 3) & ~3;
+        CU_TRY(with_type(c->type, [&](auto zero) {
+            return launch_evict(evict_kernel<decltype(zero)>, blocks, bh, static_cast<size_t>(p.range) * 8, st, p);
+        }), "evict launch");
+        return ST_OK;
+    }
     CU_TRY(with_type(c->type, [&](auto zero) {
         accumulate_kernel<decltype(zero)>
             <<<dim3(blocks_for(c->capacity, kAccThreads), bh), kAccThreads, 0, st>>>(p);
@@ -313,23 +677,8 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
     }), "accumulate launch");
     keep_kernel<<<bh, kKeepThreads, 0, st>>>(p);
     CU_TRY(cudaGetLastError(), "keep launch");
-    if (!p.keys && !p.values) return ST_OK;
-    int64_t bits = 0;
-    if (p.keys) bits |= c->key_bytes | p.kb | p.kh | p.ks | static_cast<int64_t>(reinterpret_cast<uintptr_t>(keys) & 15);
-    if (p.values) bits |= c->value_bytes | p.vb | p.vh | p.vs | static_cast<int64_t>(reinterpret_cast<uintptr_t>(values) & 15);
-    const int vec = bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
-    p.key_vecs = c->key_bytes / vec;
-    p.value_vecs = c->value_bytes / vec;
-    const int most = c->capacity - c->budget < c->budget ? c->capacity - c->budget : c->budget;
-    if (most == 0) return ST_OK;
-    const dim3 grid(blocks_for(most, 8) < 64 ? blocks_for(most, 8) : 64, bh, 2);
-    switch (vec) {
-        case 16: move_kernel<uint4><<<grid, 256, 0, st>>>(p); break;
-        case 8: move_kernel<uint2><<<grid, 256, 0, st>>>(p); break;
-        case 4: move_kernel<uint32_t><<<grid, 256, 0, st>>>(p); break;
-        case 2: move_kernel<uint16_t><<<grid, 256, 0, st>>>(p); break;
-        default: move_kernel<uint8_t><<<grid, 256, 0, st>>>(p); break;
-    }
+    if (!p.rows_vec) return ST_OK;
+    move_kernel<<<dim3(64, bh), 256, 0, st>>>(p);
     CU_TRY(cudaGetLastError(), "move launch");
     return ST_OK;
 }

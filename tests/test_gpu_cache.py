@@ -216,7 +216,7 @@ def test_a_value_buffer_alone_and_none():
             assert torch.equal(v.cpu()[0, j, :20], values[0, j, at if vb else slice(0, 20)])
 
 
-@pytest.mark.parametrize("cap", [40_000, 150_001])
+@pytest.mark.parametrize("cap", [40_000, 150_001, 196_609, 300_003])
 def test_long_caches(cap):
     g = gen(("long", cap))
     acc, pos, keys, values = make(g, 1, 2, cap, [cap - 3], dim=2)
