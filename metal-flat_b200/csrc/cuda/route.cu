@@ -254,11 +254,16 @@ __device__ __forceinline__ void load_row(const RouteParams& p, int64_t t, int la
 #pragma unroll
         for (int j = 0; j < VPL; j += N) {
             const int e = lane * VPL + j;
-            Pack<T, N> v;
-            const bool in = live && e < p.experts;
-            if (in) v = *reinterpret_cast<const Pack<T, N>*>(row + e);
+            float f[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[j + i] = in ? to_float(v.v[i]) : neg_inf();
+            for (int i = 0; i < N; ++i) f[i] = neg_inf();
+            if (live && e < p.experts) {
+                Pack<T, N> v;
+                v.load(row + e);
+                v.unpack(f);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[j + i] = f[i];
         }
     } else {
 #pragma unroll
@@ -876,10 +881,12 @@ __global__ void __launch_bounds__(kGradThreads)
     for (int j = 0; j < VPL; j += N) {
         const int e = lane * VPL + j;
         if (p.vec) {
-            Pack<T, N> v;
+            float f[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) v.v[i] = from_float<T>(d[j + i]);
-            if (e < p.experts) *reinterpret_cast<Pack<T, N>*>(row + e) = v;
+            for (int i = 0; i < N; ++i) f[i] = d[j + i];
+            Pack<T, N> v;
+            v.pack(f);
+            if (e < p.experts) v.store(row + e);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)

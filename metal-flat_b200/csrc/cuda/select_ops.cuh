@@ -29,10 +29,64 @@ __device__ __forceinline__ T from_float(float v) {
     else return v;
 }
 
-// N elements as one aligned load or store of N * sizeof(T) bytes.
+// N elements as one aligned load or store of N * sizeof(T) bytes.  (By their raw bits:
+// a struct of 16-bit floats is copied element by element.)
+template <int BYTES>
+using Raw = std::conditional_t<BYTES == 16, uint4,
+            std::conditional_t<BYTES == 8, uint2, std::conditional_t<BYTES == 4, uint32_t, uint16_t>>>;
+
 template <class T, int N>
-struct alignas(N * sizeof(T)) Pack {
-    T v[N];
+struct Pack {
+    using R = Raw<N * sizeof(T)>;
+    R raw;
+    __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const R*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<R*>(p) = raw; }
+    __device__ __forceinline__ void unpack(float (&x)[N]) const {
+        if constexpr (N * sizeof(T) == 2) {
+            x[0] = to_float(*reinterpret_cast<const T*>(&raw));
+        } else {
+            const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[i] = __uint_as_float(u[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                        x[2 * i] = __uint_as_float(u[i] << 16);
+                        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+                    } else {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                        x[2 * i] = f.x;
+                        x[2 * i + 1] = f.y;
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&x)[N]) {
+        if constexpr (N * sizeof(T) == 2) {
+            const T t = from_float<T>(x[0]);
+            raw = *reinterpret_cast<const uint16_t*>(&t);
+        } else {
+            uint32_t* u = reinterpret_cast<uint32_t*>(&raw);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) u[i] = __float_as_uint(x[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) {
+                    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                        u[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    } else {
+                        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                        u[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                }
+            }
+        }
+    }
 };
 
 // 2^t and 1/v by the special function unit, 2^-22 and 2 ulp off, subnormals flushed.
