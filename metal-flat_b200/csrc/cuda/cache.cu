@@ -46,7 +46,7 @@ struct CacheParams {
     char* keys;
     char* values;
     int vec_w, vec_a;                   // weights, and acc and pos, can be read by fours
-    int range;                          // slots of a block of evict_kernel
+    int range;                          // slots that a block of evict_kernel has room for
     int half;                           // most moves of a head: capacity / 2
     float* sums;                        // long caches [b][h][capacity]: acc'
     int32_t* holes;                     // workspace [b][h][half]
@@ -144,8 +144,7 @@ __device__ __forceinline__ void sync_blocks(uint32_t blocks) {
 }
 
 // A sum as hi + lo: every addition to hi leaves its exact rounding error (Knuth's
-// two-sum), lo adds those up.  Conversions to 64-bit floats run at about two a clock
-// and SM here: with them the sums took 54 us of a 4 x 8 x 16384 eviction's 84.
+// two-sum), lo adds those up.
 struct TwoFloats {
     float hi, lo;
     __device__ __forceinline__ void add(float x) {
@@ -157,43 +156,63 @@ struct TwoFloats {
     __device__ __forceinline__ float rounded() const { return isfinite(hi) ? hi + lo : hi; }
 };
 
+// Two of them side by side.
+struct TwoFloats2 {
+    float2 hi, lo;
+    __device__ __forceinline__ void add(float2 x) {
+        const float2 s = add2(hi, x), bb = sub2(s, hi);
+        lo = add2(lo, add2(sub2(hi, sub2(s, bb)), sub2(x, bb)));
+        hi = s;
+    }
+};
+
 constexpr int kRowsAtOnce = 8;
 
-// s[i] += the weights of slots j + i over the group's heads and `rows` query rows,
-// kRowsAtOnce rows in flight.
+// a[i] plus the weights of four adjacent slots over all rows (`rows` query rows of
+// each of the group's heads), kRowsAtOnce rows in flight; w is aligned for four.
 template <class T>
-__device__ __forceinline__ void add_rows(const T* w, int64_t wh, int64_t wq, int group, int rows, bool vec,
-                                         int most, TwoFloats (&s)[4]) {
-    int g = 0, r = 0;
-    while (g < group) {
-        if (vec) {
-            Pack<T, 4> v[kRowsAtOnce];
+__device__ __forceinline__ void add_rows(const T* w, int64_t wh, int64_t wq, int group, int rows, float (&a)[4]) {
+    TwoFloats2 s0{make_float2(a[0], a[1]), make_float2(0.0f, 0.0f)}, s1{make_float2(a[2], a[3]), make_float2(0.0f, 0.0f)};
+    const int64_t back = wh - static_cast<int64_t>(rows - 1) * wq;      // to the next head's first row
+    const int all = group * rows;
+    for (int i = 0, r = 0; i < all; i += kRowsAtOnce) {
+        Pack<T, 4> v[kRowsAtOnce];
 #pragma unroll
-            for (int u = 0; u < kRowsAtOnce; ++u) {
-                v[u].raw = {};
-                if (g < group) v[u].load(w + g * wh + r * wq);
-                if (++r == rows) {
-                    r = 0;
-                    ++g;
-                }
-            }
+        for (int u = 0; u < kRowsAtOnce; ++u) {
+            v[u].raw = {};
+            if (i + u < all) v[u].load(w);
+            const bool last = ++r == rows;
+            w += last ? back : wq;
+            r = last ? 0 : r;
+        }
 #pragma unroll
-            for (int u = 0; u < kRowsAtOnce; ++u) {
-                float x[4];
-                v[u].unpack(x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i].add(x[i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < most) s[i].add(to_float(w[g * wh + r * wq + i]));
-            if (++r == rows) {
-                r = 0;
-                ++g;
-            }
+        for (int u = 0; u < kRowsAtOnce; ++u) {
+            float x[4];
+            v[u].unpack(x);
+            s0.add(make_float2(x[0], x[1]));
+            s1.add(make_float2(x[2], x[3]));
         }
     }
+    a[0] = TwoFloats{s0.hi.x, s0.lo.x}.rounded();
+    a[1] = TwoFloats{s0.hi.y, s0.lo.y}.rounded();
+    a[2] = TwoFloats{s1.hi.x, s1.lo.x}.rounded();
+    a[3] = TwoFloats{s1.hi.y, s1.lo.y}.rounded();
+}
+
+// One slot, a warp over its rows.
+template <class T>
+__device__ __forceinline__ float add_rows_warp(const T* w, int64_t wh, int64_t wq, int group, int rows, float a) {
+    const int lane = threadIdx.x & 31;
+    TwoFloats s{lane == 0 ? a : 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = lane; i < group * rows; i += 32) s.add(to_float(w[i / rows * wh + i % rows * wq]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float hi = __shfl_xor_sync(kFullMask, s.hi, o), lo = __shfl_xor_sync(kFullMask, s.lo, o);
+        s.add(hi);
+        s.lo += lo;
+    }
+    return s.rounded();
 }
 
 // A (sequence, head): blockIdx.y; its blocks' ranges of slots: blockIdx.x, one cluster.
@@ -214,8 +233,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh % p.heads);
     const uint32_t me = blockIdx.x, blocks = gridDim.x;
     const int n = entries_of(p, b), m = min(n, p.budget);
-    const int lo = static_cast<int>(me) * p.range;
-    const int mine = max(0, min(p.range, n - lo));      // live slots of this block
+    // the live slots, spread over the blocks by fours
+    const int range = ((n + static_cast<int>(blocks) - 1) / static_cast<int>(blocks) + 3) & ~3;
+    const int lo = static_cast<int>(me) * range;
+    const int mine = max(0, min(range, n - lo));
     const float* acc = p.acc + bh * p.capacity + lo;
     const int32_t* pos = p.pos + bh * p.capacity + lo;
     float* out_acc = p.out_acc + bh * p.capacity;
@@ -225,46 +246,52 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     const int64_t since = static_cast<int64_t>(p.seen[b]) - p.recent;
 
     const int rows = !p.weights ? 0 : p.rows ? min(max(p.rows[b], 0), p.queries) : p.queries;
-    const T* weights = static_cast<const T*>(p.weights) + b * p.wb + static_cast<int64_t>(h) * p.group * p.wh + lo;
-    for (int j = threadIdx.x * 4; j < mine; j += kEvictThreads * 4) {
-        const int most = min(4, mine - j);
-        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        int q[4] = {0, 0, 0, 0};
-        if (p.vec_a && most == 4) {
+    const T* weights = rows > 0 ? static_cast<const T*>(p.weights) + b * p.wb + static_cast<int64_t>(h) * p.group * p.wh + lo : nullptr;
+    auto put = [&](int j, float a, int q) {
+        if (over) {
+            sums[j] = a;
+            keys[j] = slot_key(p, a, q, since);
+        } else {
+            out_acc[lo + j] = a;
+            out_pos[lo + j] = q;
+        }
+    };
+    // whole fours, a thread each; then the slots behind them, or all where the weights
+    // are not aligned for it
+    const int fours = p.vec_w ? mine & ~3 : 0;
+    for (int j = threadIdx.x * 4; j < fours; j += kEvictThreads * 4) {
+        float a[4];
+        int q[4];
+        if (p.vec_a) {
             const float4 va = *reinterpret_cast<const float4*>(acc + j);
             const int4 vq = *reinterpret_cast<const int4*>(pos + j);
             a[0] = va.x, a[1] = va.y, a[2] = va.z, a[3] = va.w;
             q[0] = vq.x, q[1] = vq.y, q[2] = vq.z, q[3] = vq.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < most) {
-                    a[i] = acc[j + i];
-                    q[i] = pos[j + i];
-                }
+            for (int i = 0; i < 4; ++i) {
+                a[i] = acc[j + i];
+                q[i] = pos[j + i];
+            }
         }
-        if (rows > 0) {
-            TwoFloats s[4];
+        if (rows > 0) add_rows(weights + j, p.wh, p.wq, p.group, rows, a);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = TwoFloats{a[i], 0.0f};
-            add_rows(weights + j, p.wh, p.wq, p.group, rows, p.vec_w && most == 4, most, s);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = s[i].rounded();
+        for (int i = 0; i < 4; ++i) put(j + i, a[i], q[i]);
+    }
+    if (p.group * rows < 16 || fours == 0) {
+        // (few rows, or many slots: a thread each)
+        for (int j = fours + threadIdx.x; j < mine; j += kEvictThreads) {
+            TwoFloats s{acc[j], 0.0f};
+            const T* w = weights + j;
+            for (int g = 0; g < p.group && rows > 0; ++g)
+#pragma unroll 8
+                for (int r = 0; r < rows; ++r) s.add(to_float(w[g * p.wh + r * p.wq]));
+            put(j, s.rounded(), pos[j]);
         }
-        if (over) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < most) {
-                    sums[j + i] = a[i];
-                    keys[j + i] = slot_key(p, a[i], q[i], since);
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < most) {
-                    out_acc[lo + j + i] = a[i];
-                    out_pos[lo + j + i] = q[i];
-                }
+    } else {
+        for (int j = fours + static_cast<int>(threadIdx.x >> 5); j < mine; j += kEvictWarps) {
+            const float a = add_rows_warp(weights + j, p.wh, p.wq, p.group, rows, acc[j]);
+            if ((threadIdx.x & 31) == 0) put(j, a, pos[j]);
         }
     }
     if (!over) return;
