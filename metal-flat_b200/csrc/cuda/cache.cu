@@ -25,6 +25,7 @@ namespace {
 constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictSlots = 24576;      // slots a block holds, 8 bytes each
 constexpr int kEvictCluster = 8;
+constexpr int kGather = 2048;           // keys of one digit that a block takes in
 constexpr int kAccThreads = 256;
 constexpr int kKeepThreads = 512, kKeepWarps = kKeepThreads / 32;
 
@@ -45,7 +46,7 @@ struct CacheParams {
     int32_t* out_lens;
     char* keys;
     char* values;
-    int vec_w, vec_a;                   // weights, and acc and pos, can be read by fours
+    int vec_w, vec_a;                   // weights, and acc and pos, can be moved by fours
     int range;                          // slots that a block of evict_kernel has room for
     int half;                           // most moves of a head: capacity / 2
     float* sums;                        // long caches [b][h][capacity]: acc'
@@ -222,11 +223,12 @@ __device__ __forceinline__ float add_rows_warp(const T* w, int64_t wh, int64_t w
 // a run of adjacent slots, so that one scan over the threads orders all of them.
 template <class T>
 __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CacheParams p) {
-    extern __shared__ uint32_t dyn[];
+    extern __shared__ __align__(16) uint32_t dyn[];
     __shared__ __align__(16) int hist[2][2048];
     __shared__ int warp_sum[kEvictWarps];
     __shared__ uint32_t sh_prefix;
-    __shared__ int sh_left, sh_ties, sh_moves;
+    __shared__ __align__(16) int small[128];
+    __shared__ int sh_left, sh_share, sh_own, sh_ties, sh_moves;
     uint32_t* keys = dyn;
     float* sums = reinterpret_cast<float*>(dyn + p.range);
     const int64_t bh = blockIdx.y;
@@ -247,13 +249,15 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
 
     const int rows = !p.weights ? 0 : p.rows ? min(max(p.rows[b], 0), p.queries) : p.queries;
     const T* weights = rows > 0 ? static_cast<const T*>(p.weights) + b * p.wb + static_cast<int64_t>(h) * p.group * p.wh + lo : nullptr;
+    // slots below m keep their place unless they turn out to be holes: written at once
     auto put = [&](int j, float a, int q) {
+        if (lo + j < m) {
+            out_acc[lo + j] = a;
+            out_pos[lo + j] = q;
+        }
         if (over) {
             sums[j] = a;
             keys[j] = slot_key(p, a, q, since);
-        } else {
-            out_acc[lo + j] = a;
-            out_pos[lo + j] = q;
         }
     };
     // whole fours, a thread each; then the slots behind them, or all where the weights
@@ -275,8 +279,21 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
             }
         }
         if (rows > 0) add_rows(weights + j, p.wh, p.wq, p.group, rows, a);
+        if (p.vec_a && (lo + j + 4 <= m || lo + j >= m)) {
+            if (lo + j < m) {
+                *reinterpret_cast<float4*>(out_acc + lo + j) = make_float4(a[0], a[1], a[2], a[3]);
+                *reinterpret_cast<int4*>(out_pos + lo + j) = make_int4(q[0], q[1], q[2], q[3]);
+            }
+            if (over) {
+                *reinterpret_cast<float4*>(sums + j) = make_float4(a[0], a[1], a[2], a[3]);
+                *reinterpret_cast<uint4*>(keys + j) =
+                    make_uint4(slot_key(p, a[0], q[0], since), slot_key(p, a[1], q[1], since),
+                               slot_key(p, a[2], q[2], since), slot_key(p, a[3], q[3], since));
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put(j + i, a[i], q[i]);
+            for (int i = 0; i < 4; ++i) put(j + i, a[i], q[i]);
+        }
     }
     if (p.group * rows < 16 || fours == 0) {
         // (few rows, or many slots: a thread each)
@@ -296,10 +313,14 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     }
     if (!over) return;
 
-    if (threadIdx.x == 0) { sh_prefix = 0; sh_left = m; }
+    if (threadIdx.x == 0) { sh_prefix = 0; sh_left = m; sh_own = 0; }
     for (int i = threadIdx.x; i < 2048; i += kEvictThreads) hist[0][i] = 0;
     __syncthreads();
+    // The m-th key: its first 11 bits by a histogram over the cluster.  The keys that
+    // share them, few as a rule, are gathered by every block, which finds the other
+    // 21 bits alone; more of them than a block takes in go on over the cluster.
     uint32_t mask = 0;
+    bool alone = false;
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
@@ -325,9 +346,6 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
                 }
         }
         const int count[4] = {c.w, c.z, c.y, c.x}, sum = c.x + c.y + c.z + c.w;
-        // (read by the other blocks before this pass's cluster barrier)
-        if (pass < 2)
-            for (int i = threadIdx.x; i < 2048; i += kEvictThreads) hist[(pass + 1) & 1][i] = 0;
         const int left = sh_left;
         int total;
         int above = scan_block(sum, warp_sum, total);       // its barriers: left is read
@@ -336,11 +354,75 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
             if (above < left && left <= above + count[i]) {
                 sh_prefix = prefix | (static_cast<uint32_t>(2047 - (threadIdx.x * 4 + i)) << shift);
                 sh_left = left - above;
+                sh_share = count[i];
             }
             above += count[i];
         }
         mask |= digits << shift;
         __syncthreads();
+        if (pass == 0 && sh_share <= kGather) {
+            alone = true;
+            break;
+        }
+        // (read by the other blocks before this pass's cluster barrier)
+        if (pass < 2) {
+            for (int i = threadIdx.x; i < 2048; i += kEvictThreads) hist[(pass + 1) & 1][i] = 0;
+            __syncthreads();
+        }
+    }
+    if (alone) {
+        // hist[1] takes this block's keys, then hist[0] all blocks'
+        uint32_t* own = reinterpret_cast<uint32_t*>(hist[1]);
+        const uint32_t prefix = sh_prefix;
+        for (int j = threadIdx.x; j < mine; j += kEvictThreads)
+            if ((keys[j] & mask) == prefix) own[atomicAdd(&sh_own, 1)] = keys[j];
+        sync_blocks(blocks);
+        const uint32_t* all = own;
+        const int n_all = sh_share;
+        if (blocks > 1) {
+            uint32_t* got = reinterpret_cast<uint32_t*>(hist[0]);
+            int base = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < kEvictCluster; ++r)
+                if (r < blocks) {
+                    const int c = cluster_load(&sh_own, r);
+                    for (int i = threadIdx.x; i < c; i += kEvictThreads)
+                        got[base + i] = static_cast<uint32_t>(cluster_load(reinterpret_cast<int*>(own + i), r));
+                    base += c;
+                }
+            all = got;
+        }
+        for (int shift = 14; shift >= 0; shift -= 7) {
+            if (threadIdx.x < 128) small[threadIdx.x] = 0;
+            __syncthreads();
+            const uint32_t prefix = sh_prefix;
+            for (int i = threadIdx.x; i < n_all; i += kEvictThreads)
+                if ((all[i] & mask) == prefix) atomicAdd(&small[(all[i] >> shift) & 127u], 1);
+            __syncthreads();
+            if (threadIdx.x < 32) {
+                // four digits a lane, from the top down
+                const int lane = threadIdx.x;
+                const int4 c = *reinterpret_cast<const int4*>(&small[124 - 4 * lane]);
+                const int count[4] = {c.w, c.z, c.y, c.x}, sum = c.x + c.y + c.z + c.w, left = sh_left;
+                int above = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(kFullMask, above, o);
+                    if (lane >= o) above += u;
+                }
+                above -= sum;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (above < left && left <= above + count[i]) {
+                        sh_prefix = prefix | (static_cast<uint32_t>(127 - (4 * lane + i)) << shift);
+                        sh_left = left - above;
+                    }
+                    above += count[i];
+                }
+            }
+            mask |= 127u << shift;
+            __syncthreads();
+        }
     }
     const uint32_t cut = sh_prefix;
     const int ties = sh_left;           // entries at the cut that stay, the lowest slots
@@ -379,7 +461,6 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     for (int j = j0; j < j1; ++j) {
         const uint32_t key = keys[j];
         const bool keep = key > cut || (key == cut && tie++ < ties);
-        keys[j] = keep ? 1u : 0u;
         if (lo + j < m) {
             if (!keep) holes[hole++] = lo + j;
         } else if (keep) {
@@ -389,11 +470,6 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
         }
     }
     sync_blocks(blocks);                // the lists are complete and in every block's sight
-    for (int j = threadIdx.x; j < mine && lo + j < m; j += kEvictThreads)
-        if (keys[j]) {
-            out_acc[lo + j] = sums[j];
-            if (p.out_pos != p.pos) out_pos[lo + j] = pos[j];
-        }
     const int at = static_cast<int>(me) * kEvictThreads + threadIdx.x, step = static_cast<int>(blocks) * kEvictThreads;
     for (int i = at; i < moves; i += step) {
         const int to = holes[i];
@@ -694,7 +770,8 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
     p.tail_pos = reinterpret_cast<int32_t*>(w + l.tail_pos);
     p.half = c->capacity / 2;
     p.vec_w = ((p.wb | p.wh | p.wq) & 3) == 0 && aligned_to(weights, 4 * type_bytes(c->type));
-    p.vec_a = (c->capacity & 3) == 0 && aligned_to(acc, 16) && aligned_to(pos, 16);
+    p.vec_a = (c->capacity & 3) == 0 && aligned_to(acc, 16) && aligned_to(pos, 16) &&
+              aligned_to(out_acc, 16) && aligned_to(out_pos, 16);
     int64_t bits = 0;
     if (p.keys) bits |= c->key_bytes | p.kb | p.kh | p.ks | static_cast<int64_t>(reinterpret_cast<uintptr_t>(keys) & 15);
     if (p.values) bits |= c->value_bytes | p.vb | p.vh | p.vs | static_cast<int64_t>(reinterpret_cast<uintptr_t>(values) & 15);
