@@ -810,17 +810,9 @@ __global__ void __launch_bounds__(kGradThreads)
         if (id < 0 || id >= p.experts) id = -1;
         else g = grad[t * p.k + lane];
     }
-    // the logit of each chosen expert, from the lane that holds it
     float xid = neg_inf();
-    for (int r = 0; r < p.k; ++r) {
-        const int e = __shfl_sync(kFullMask, id, base + r);
-        float v = neg_inf();
-#pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (e == lane * VPL + j) v = x[j];
-        v = __shfl_sync(kFullMask, v, base + (e < 0 ? 0 : e / VPL));
-        if (lane == r) xid = v;
-    }
+    if (id >= 0) xid = to_float(static_cast<const T*>(p.logits)[t * p.stride + id]);
+    if (!(xid > neg_inf())) xid = neg_inf();
     const bool chosen = id >= 0 && xid > neg_inf();
     if (!chosen) g = 0.0f;
     float d[VPL], m = 0.0f, sum = 1.0f;
@@ -847,9 +839,9 @@ __global__ void __launch_bounds__(kGradThreads)
     const float w = weight_of(q, chosen, xid, m, sum);
     const float dot = (p.softmax || p.renormalise) ? lane_sum<LPT>(g * w) : 0.0f;
     if (whole) {
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = sum > 0.0f ? p.scale * inverse_fast(sum) : 0.0f;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) d[j] *= inv * p.scale;
+        for (int j = 0; j < VPL; ++j) d[j] *= inv;
         float mult[VPL];
 #pragma unroll
         for (int j = 0; j < VPL; ++j) mult[j] = -dot;
@@ -864,7 +856,7 @@ __global__ void __launch_bounds__(kGradThreads)
         for (int j = 0; j < VPL; ++j) d[j] *= mult[j];
     } else {
         float v = p.scale * w * (p.renormalise ? g - dot : g);
-        if (!p.softmax) v *= 1.0f / (1.0f + expf(xid));   // 1 - s
+        if (!p.softmax) v *= inverse_fast(1.0f + expf(xid));    // 1 - s
         if (!chosen) v = 0.0f;
         for (int r = 0; r < p.k; ++r) {
             const int e = __shfl_sync(kFullMask, id, base + r);
@@ -911,14 +903,21 @@ cudaError_t with_layout(int experts, Fn&& fn) {
     return fn(integral_constant<int, 32>{}, integral_constant<int, 32>{}, integral_constant<int, 256>{});
 }
 
-int pack_elems(int experts, size_t es) {   // elements of one load of load_row()
-    int vpl = 1;
-    while (vpl * 32 < experts) vpl *= 2;
-    return vpl * es >= 16 ? static_cast<int>(16 / es) : vpl;
+// The gradient's layout: 8 experts a lane (16 bytes of 16-bit logits), so that up to
+// four tokens share a warp and its exchanges; else as above.
+template <class Fn>
+cudaError_t with_grad_layout(int experts, int k, Fn&& fn) {
+    using std::integral_constant;
+    const integral_constant<int, 8> eight{};
+    if (experts > 32 && experts <= 64 && k <= 8) return fn(eight, eight);
+    if (experts > 32 && experts <= 128 && k <= 16) return fn(integral_constant<int, 16>{}, eight);
+    return with_layout(experts, [&](auto lpt, auto vpl, auto) { return fn(lpt, vpl); });
 }
 
-bool packed_rows(const void* p, int64_t stride, int experts, size_t es) {
-    const size_t n = pack_elems(experts, es);
+// Whether rows can be moved in whole packs of 16 bytes, or of a lane's vpl experts
+// where those are less.
+bool packed_rows(const void* p, int64_t stride, int experts, int vpl, size_t es) {
+    const size_t n = vpl * es >= 16 ? 16 / es : static_cast<size_t>(vpl);
     return experts % n == 0 && stride % static_cast<int64_t>(n) == 0 && aligned_to(p, n * es);
 }
 
@@ -995,11 +994,11 @@ int fill_params(const mflat_cu_router_t* r, const void* logits, int64_t& stride,
     p.groups_kept = r->groups_kept;
     p.group_top = r->group_top;
     p.scale = r->scale;
-    p.vec = packed_rows(logits, stride, r->experts, type_bytes(r->type));
     p.k_lanes = 1;
     while (p.k_lanes < r->k) p.k_lanes *= 2;
     int vpl = 1;
     while (vpl * 32 < r->experts) vpl *= 2;
+    p.vec = packed_rows(logits, stride, r->experts, vpl, type_bytes(r->type));
     const int size = r->experts / r->groups;
     const int lanes = size % vpl == 0 ? size / vpl : 0;
     p.lane_groups = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
@@ -1090,12 +1089,16 @@ extern "C" int mflat_cu_route_backward(const mflat_cu_router_t* r, const void* l
     if (rc != ST_OK) return rc;
     DeviceGuard g(device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    p.vec = p.vec && packed_rows(grad, grad_stride, r->experts, type_bytes(r->type));
+    const size_t es = type_bytes(r->type);
+    auto vec_for = [&](int vpl) {
+        return packed_rows(logits, stride, r->experts, vpl, es) && packed_rows(grad, grad_stride, r->experts, vpl, es);
+    };
     p.ids = const_cast<int32_t*>(ids);
     CU_TRY(with_type(r->type, [&](auto zero) {
         using T = decltype(zero);
-        return with_layout(r->experts, [&](auto lpt, auto vpl, auto) {
+        return with_grad_layout(r->experts, r->k, [&](auto lpt, auto vpl) {
             constexpr int L = decltype(lpt)::value, V = decltype(vpl)::value;
+            p.vec = vec_for(V);
             route_backward_kernel<T, L, V>
                 <<<blocks_for(static_cast<int64_t>(tokens) * L, kGradThreads), kGradThreads, 0, st>>>(
                     p, grad_weights, static_cast<T*>(grad), grad_stride);
