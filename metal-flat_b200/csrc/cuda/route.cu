@@ -107,6 +107,27 @@ __device__ __forceinline__ S lane_sum(S v) {
 
 // Scores of the lane's experts, lane l of a token holding experts
 // [l * VPL, (l + 1) * VPL).  x: fp32 logits, -inf for "none".
+// e[j] = exp(x[j] - m), m the row's largest: 0 for -inf, and where m itself is infinite 1
+// for the logits that are m.  Returns the lane's sum.
+template <class S, int VPL>
+__device__ __forceinline__ S exps_of(const float (&x)[VPL], float m, S (&e)[VPL]) {
+    S sum = 0;
+    if (fabsf(m) < -neg_inf()) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            e[j] = exp_of<S>(S(x[j]) - S(m));
+            sum += e[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+            e[j] = x[j] == m && m > 0.0f ? S(1) : S(0);
+            sum += e[j];
+        }
+    }
+    return sum;
+}
+
 template <class S>
 __device__ __forceinline__ S inverse(S v) {
     if constexpr (sizeof(S) == 4) return inverse_fast(v);
@@ -121,13 +142,7 @@ __device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S
         for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
 #pragma unroll
         for (int o = LPT / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-        S sum = 0;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            s[j] = x[j] == neg_inf() ? S(0) : x[j] == m ? S(1) : exp_of<S>(S(x[j]) - S(m));
-            sum += s[j];
-        }
-        sum = lane_sum<LPT>(sum);
+        const S sum = lane_sum<LPT>(exps_of<S, VPL>(x, m, s));
         const S inv = sum > S(0) ? inverse(sum) : S(0);
         largest = inv;
 #pragma unroll
@@ -358,7 +373,7 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
     float a = none, b = none;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        const float v = key[j] > none ? c[j] : none;
+        const float v = c[j];       // -inf where there is no choice; NaN passes by
         b = fmaxf(b, fminf(a, v));
         a = fmaxf(a, v);
     }
@@ -375,18 +390,22 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
     if (exact) tau = 0.0f;
     const int base = (threadIdx.x & 31) - lane;
     const int group = lane / p.lane_groups;
-    // groups above for sure, and those not below for sure (itself among them)
-    int above = 0, near = 0;
+    // groups above for sure, and those not below for sure (itself among them): the lanes
+    // of a group share the comparisons; counts in half words
+    int counts = 0;
     const float high = mine + tau, low = mine - tau;
-    for (int g = 0; g < p.groups; ++g) {
-        const float v = __shfl_sync(kFullMask, mine, base + g * p.lane_groups);
+    for (int g0 = 0; g0 < p.groups; g0 += p.lane_groups) {
+        const int g = g0 + (lane & (p.lane_groups - 1));
+        const float v = __shfl_sync(kFullMask, mine, base + min(g, p.groups - 1) * p.lane_groups);
+        if (g >= p.groups) continue;
         if constexpr (exact) {
-            above += v > mine || (v == mine && g < group) ? 1 : 0;
+            counts += v > mine || (v == mine && g < group) ? 1 : 0;
         } else {
-            above += v > high ? 1 : 0;
-            near += !(v < low) ? 1 : 0;
+            counts += (v > high ? 1 : 0) + (v < low ? 0 : 1 << 16);
         }
     }
+    for (int o = 1; o < p.lane_groups; o <<= 1) counts += __shfl_xor_sync(kFullMask, counts, o);
+    const int above = counts & 0xffff, near = counts >> 16;
     const bool kept = exact ? above < p.groups_kept : near <= p.groups_kept;
     const bool dropped = above >= p.groups_kept || mine == none;
     if (!kept) {
@@ -397,7 +416,9 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
 }
 
 // A warp's scratch for one token's candidates.
+template <int VPL>
 struct RouteScratch {
+    float keys[VPL * 32];               // [j][lane]
     float2 cand[kCandMax];              // key, expert
     float2 best[kMaxRouteK + 1];
 };
@@ -405,7 +426,7 @@ struct RouteScratch {
 // The choice scores of a token's n candidates in 64 bits, lane l those of candidates
 // l and l + 32.  The row is read again, so that the common path keeps its registers.
 template <class T>
-__device__ __noinline__ void refine(const RouteParams& p, const T* row, const RouteScratch& sh, int n,
+__device__ __noinline__ void refine(const RouteParams& p, const T* row, const float2* cand, int n,
                                     double (&c)[2]) {
     const int lane = threadIdx.x & 31;
     double m = 0.0, sum = 1.0;
@@ -427,7 +448,7 @@ __device__ __noinline__ void refine(const RouteParams& p, const T* row, const Ro
         const int i = lane + 32 * h;
         c[h] = static_cast<double>(neg_inf());
         if (i < n) {
-            const int e = __float_as_int(sh.cand[i].y);
+            const int e = __float_as_int(cand[i].y);
             const double v = to_float(row[e]);
             const double s = p.softmax ? (v == m ? 1.0 : exp(v - m)) / sum : 1.0 / (1.0 + exp(-v));
             c[h] = s + static_cast<double>(p.bias[e]);
@@ -443,7 +464,7 @@ __device__ __noinline__ void refine(const RouteParams& p, const T* row, const Ro
 template <class T, int VPL>
 __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* row, const float (&key)[VPL],
                                                float base_tau,
-                                               RouteScratch& sh, int& id) {
+                                               RouteScratch<VPL>& sh, int& id) {
     const int lane = threadIdx.x & 31, k = p.k;
     const bool check = p.bias != nullptr;
     float top = key[0];
@@ -453,10 +474,12 @@ __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* ro
     if (k <= 8) {
         // k maxima, each with all its equals taken out: 3 instructions each
         uint32_t v = choice_key(top), m = 0;
-        for (int r = 0; r < k; ++r) {
-            m = __reduce_max_sync(kFullMask, v);
-            v = v == m ? 0u : v;
-        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (r < k) {
+                m = __reduce_max_sync(kFullMask, v);
+                v = v == m ? 0u : v;
+            }
         floor_v = key_value(m);
     } else {
         float v = top;
@@ -471,17 +494,27 @@ __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* ro
         floor_v = __shfl_sync(kFullMask, v, k - 1);
     }
     if (check) floor_v -= tau_of(base_tau, floor_v);
-    const unsigned below = (1u << lane) - 1u;
-    int n = 0;
+    // few lanes have any: those list theirs one after the other, behind the lanes below
+    uint32_t mine_bits = 0;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        const bool in = !(key[j] < floor_v) && key[j] > neg_inf();
-        const unsigned who = __ballot_sync(kFullMask, in);
-        const int at = n + __popc(who & below);
-        if (in && at < kCandMax) sh.cand[at] = make_float2(key[j], __int_as_float(lane * VPL + j));
-        n += __popc(who);
+        sh.keys[j * 32 + lane] = key[j];
+        if (key[j] >= floor_v && key[j] > neg_inf()) mine_bits |= 1u << j;
+    }
+    const int count = __popc(mine_bits);
+    int at = 0, n = 0;
+#pragma unroll
+    for (int s = 0; (1 << s) <= VPL; ++s) {
+        const unsigned who = __ballot_sync(kFullMask, (count >> s) & 1);
+        at += __popc(who & ((1u << lane) - 1u)) << s;
+        n += __popc(who) << s;
     }
     if (n > kCandMax) return true;
+    while (mine_bits) {
+        const int j = __ffs(mine_bits) - 1;
+        mine_bits &= mine_bits - 1u;
+        sh.cand[at++] = make_float2(sh.keys[j * 32 + lane], __int_as_float(lane * VPL + j));
+    }
     __syncwarp();
     for (int i = lane; i < n; i += 32) {
         const float2 c = sh.cand[i];
@@ -504,7 +537,7 @@ __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* ro
         const bool close = lane < k && next > neg_inf() && !(mine.x - next > tau_of(base_tau, mine.x));
         if (__any_sync(kFullMask, close)) {
             double c[2];
-            refine<T>(p, row, sh, n, c);
+            refine<T>(p, row, sh.cand, n, c);
             __syncwarp();
             id = -1;
 #pragma unroll
@@ -567,7 +600,8 @@ __device__ __forceinline__ void block_exclusive(int* v, int n, int* warp_sum) {
 template <class T, int LPT, int VPL, int NT>
 __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ RouteParams p) {
     constexpr int kWarps = NT / 32, kAtOnce = NT / LPT, kMost = LPT * VPL;
-    __shared__ RouteScratch scratch[VPL > 1 ? kWarps : 1];
+    extern __shared__ __align__(16) char dyn[];
+    RouteScratch<VPL>* scratch = reinterpret_cast<RouteScratch<VPL>*>(dyn);
     const int lane = threadIdx.x % LPT, warp = threadIdx.x >> 5;
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
     const int64_t t1 = max(t0, min(t0 + p.tile, static_cast<int64_t>(p.tokens)));
@@ -591,11 +625,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
             for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
 #pragma unroll
             for (int o = LPT / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-            sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                sum += x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : exp_of<float>(x[j] - m);
-            sum = lane_sum<LPT>(sum);
+            sum = lane_sum<LPT>(exps_of<float, VPL>(x, m, key));
         }
         bool doubt = false;
         float base_tau = 0.0f;
@@ -605,9 +635,9 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
             base_tau = tau_base(p.softmax, largest, VPL);
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                c[j] += b[j];
                 // (a bias of NaN makes a key that no comparison takes)
-                key[j] = !p.bias ? x[j] : x[j] > neg_inf() ? c[j] : neg_inf();
+                c[j] = x[j] > neg_inf() ? c[j] + b[j] : neg_inf();
+                key[j] = p.bias ? c[j] : x[j];
             }
             if (p.groups > 1) doubt = choose_groups<LPT, VPL, false>(p, lane, c, base_tau, key);
         } else {
@@ -757,6 +787,15 @@ __global__ void __launch_bounds__(kListThreads) lists_kernel(const __grid_consta
     }
     __syncthreads();
     grid_wait();
+    // the thread's first choice is on its way while the counts are summed
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
+    const int64_t t1 = min(t0 + p.tile, static_cast<int64_t>(p.tokens));
+    const int64_t first = t0 * p.k + threadIdx.x;
+    int id0 = -1, rank0 = 0;
+    if (first < t1 * p.k) {
+        id0 = p.ids[first];
+        rank0 = p.ranks[first];
+    }
     const int pair = threadIdx.x % pairs, group = threadIdx.x / pairs;
     if (group < groups) {
         int b0 = 0, b1 = 0, s0 = 0, s1 = 0;
@@ -782,9 +821,8 @@ __global__ void __launch_bounds__(kListThreads) lists_kernel(const __grid_consta
     block_exclusive<kListThreads>(total, p.experts + 1, warp_sum);
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e <= p.experts; e += kListThreads) p.start[e] = total[e];
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
-    const int64_t t1 = min(t0 + p.tile, static_cast<int64_t>(p.tokens));
-    for (int64_t i = t0 * p.k + threadIdx.x; i < t1 * p.k; i += kListThreads) {
+    if (id0 >= 0) p.slots[total[id0] + before[id0] + rank0] = static_cast<int32_t>(first);
+    for (int64_t i = first + kListThreads; i < t1 * p.k; i += kListThreads) {
         const int id = p.ids[i];
         if (id >= 0) p.slots[total[id] + before[id] + p.ranks[i]] = static_cast<int32_t>(i);
     }
@@ -823,13 +861,7 @@ __global__ void __launch_bounds__(kGradThreads)
         for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
 #pragma unroll
         for (int o = LPT / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-        sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            d[j] = x[j] == neg_inf() ? 0.0f : x[j] == m ? 1.0f : exp_of<float>(x[j] - m);
-            sum += d[j];
-        }
-        sum = lane_sum<LPT>(sum);
+        sum = lane_sum<LPT>(exps_of<float, VPL>(x, m, d));
     } else {
 #pragma unroll
         for (int j = 0; j < VPL; ++j) d[j] = 0.0f;
@@ -885,6 +917,29 @@ __global__ void __launch_bounds__(kGradThreads)
                 if (e + i < p.experts) row[e + i] = from_float<T>(d[j + i]);
         }
     }
+}
+
+// One block a tile, all in one cluster or on their own.
+template <class K>
+cudaError_t launch_route(K kernel, unsigned threads, size_t smem, cudaStream_t st, const RouteParams& p) {
+    if (smem > 0) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.tiles));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = static_cast<unsigned>(p.tiles);
+    at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = p.cluster ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 // Calls fn(LPT, VPL, NT) as integral constants for a router: as few lanes per
@@ -1059,9 +1114,8 @@ extern "C" int mflat_cu_route(const mflat_cu_router_t* r, const void* logits, in
         using T = decltype(zero);
         return with_layout(r->experts, [&](auto lpt, auto vpl, auto nt) {
             constexpr int L = decltype(lpt)::value, V = decltype(vpl)::value, N = decltype(nt)::value;
-            if (p.cluster) return launch_cluster(route_kernel<T, L, V, N>, p.tiles, N, st, p);
-            route_kernel<T, L, V, N><<<p.tiles, N, 0, st>>>(p);
-            return cudaGetLastError();
+            constexpr size_t smem = V > 1 ? sizeof(RouteScratch<V>) * (N / 32) : 0;
+            return launch_route(route_kernel<T, L, V, N>, N, smem, st, p);
         });
     }), "route launch");
     if (start && !l.cluster)

@@ -168,24 +168,6 @@ cudaError_t launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-// All blocks of the grid as one cluster.
-template <class... P, class... A>
-cudaError_t launch_cluster(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t st,
-                           A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = blocks;
-    at.val.clusterDim.y = 1;
-    at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
 inline size_t type_bytes(int type) { return type == 0 ? 4 : 2; }
 inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 
