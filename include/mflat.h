@@ -311,7 +311,8 @@ typedef struct {
 
 MFLAT_API size_t mflat_beam_workspace_bytes(const mflat_beam_t*, int batch);
 /* d_logits: (batch * beams) rows of vocab; d_cum, d_finished (nullable): batch x
- * beams.  Outputs batch x k: parent beam, token, new cum; -1 / -1 / -inf padded. */
+ * beams.  Outputs batch x k: parent beam, token, new cum; -1 / -1 / -inf padded.
+ * d_out_scores may be d_cum where k = beams. */
 MFLAT_API mflat_status_t mflat_beam_select_device(const mflat_beam_t*, const void* d_logits,
         int64_t stride, const float* d_cum, const uint8_t* d_finished, int batch,
         int32_t* d_out_parents, int32_t* d_out_tokens, float* d_out_scores,
@@ -335,7 +336,7 @@ MFLAT_API mflat_status_t mflat_beam_reorder_device(void* d_states, const int32_t
  * positions' order, d_pos tells them. */
 typedef struct {
     int heads, group;               /* cache heads; query heads per cache head      */
-    int capacity;                   /* slots per (sequence, head)                   */
+    int capacity;                   /* slots per (sequence, head), at most 2^30     */
     int budget, recent, sink;       /* sink + recent <= budget <= capacity          */
     mflat_storage_t type;           /* of the attention weights                     */
     int64_t key_bytes, value_bytes; /* one entry's row; 0 = no such buffer          */

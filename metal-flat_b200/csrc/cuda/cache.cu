@@ -13,6 +13,7 @@
 // The three kernels behind it are for caches longer than eight blocks hold.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdio>
 
@@ -25,6 +26,7 @@ namespace {
 constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictSlots = 24576;      // slots a block holds, 8 bytes each
 constexpr int kEvictCluster = 8;
+constexpr int kMaxCapacity = 1 << 30;
 constexpr int kGather = 2048;           // keys of one digit that a block takes in
 constexpr int kAccThreads = 256;
 constexpr int kKeepThreads = 512, kKeepWarps = kKeepThreads / 32;
@@ -651,8 +653,8 @@ CacheLayout cache_layout(const mflat_cu_cache_t* c, int batch) {
 
 int check_cache(const mflat_cu_cache_t* c, int batch) {
     char msg[200];
-    if (c->heads < 1 || c->group < 1 || c->capacity < 1)
-        return fail(ST_BAD_ARG, "heads, group and capacity must be at least 1");
+    if (c->heads < 1 || c->group < 1 || c->capacity < 1 || c->capacity > kMaxCapacity)
+        return fail(ST_BAD_ARG, "heads and group must be at least 1, capacity in [1, 2^30]");
     if (c->budget < 1 || c->budget > c->capacity || c->recent < 0 || c->sink < 0 ||
         static_cast<int64_t>(c->recent) + c->sink > c->budget) {
         std::snprintf(msg, sizeof msg, "budget=%d recent=%d sink=%d: need 0 <= sink + recent <= budget <= "
@@ -689,9 +691,10 @@ cudaError_t launch_evict(K kernel, int blocks, unsigned bh, size_t smem, cudaStr
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-// Dense strides where all are 0; false where two rows could overlap.
-bool fill_strides(const int64_t* s, int64_t bytes, int heads, int capacity, int64_t& sb, int64_t& sh,
-                  int64_t& ss) {
+// Dense strides where all are 0; false where two rows could overlap: the smallest
+// stride has to span a row, each larger one all of what the one below it steps over.
+bool fill_strides(const int64_t* s, int64_t bytes, int64_t batch, int heads, int capacity, int64_t& sb,
+                  int64_t& sh, int64_t& ss) {
     sb = s[0];
     sh = s[1];
     ss = s[2];
@@ -700,7 +703,20 @@ bool fill_strides(const int64_t* s, int64_t bytes, int heads, int capacity, int6
         sh = ss * capacity;
         sb = sh * heads;
     }
-    return ss >= bytes && sh >= bytes && sb >= bytes;
+    if (sb < 0 || sh < 0 || ss < 0) return false;
+    if (bytes == 0) return true;
+    struct Dim {
+        __int128 stride;
+        int64_t count;
+    } dims[3] = {{sb, batch}, {sh, heads}, {ss, capacity}};
+    std::sort(dims, dims + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    __int128 span = bytes;
+    for (const Dim& d : dims) {
+        if (d.count <= 1) continue;
+        if (d.stride < span) return false;
+        span = d.stride * d.count;
+    }
+    return span <= (static_cast<__int128>(1) << 56);
 }
 
 }  // namespace
@@ -721,7 +737,8 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
                                     void* ws, size_t ws_bytes, int device, void* stream) {
     int rc = check_cache(c, batch);
     if (rc != ST_OK) return rc;
-    if (weights && queries < 0) return fail(ST_BAD_ARG, "queries below 0");
+    if (weights && (queries < 0 || static_cast<int64_t>(c->group) * queries > INT_MAX))
+        return fail(ST_BAD_ARG, "queries below 0, or group * queries of 2^31 or more");
     CacheParams p{};
     p.heads = c->heads;
     p.group = c->group;
@@ -736,13 +753,15 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
         p.wq = weight_stride[2];
         if (p.wb < 0 || p.wh < 0 || p.wq < 0) return fail(ST_BAD_ARG, "negative weight stride");
     } else {
+        const __int128 span = static_cast<__int128>(c->capacity) * queries * c->heads * c->group;
+        if (weights && span > (static_cast<__int128>(1) << 56)) return fail(ST_BAD_ARG, "weights span more than 2^56");
         p.wq = c->capacity;
-        p.wh = p.wq * queries;
-        p.wb = p.wh * c->heads * c->group;
+        p.wh = weights ? p.wq * queries : 0;
+        p.wb = weights ? p.wh * c->heads * c->group : 0;
     }
-    if (!fill_strides(c->key_stride, c->key_bytes, c->heads, c->capacity, p.kb, p.kh, p.ks) ||
-        !fill_strides(c->value_stride, c->value_bytes, c->heads, c->capacity, p.vb, p.vh, p.vs))
-        return fail(ST_BAD_ARG, "cache strides below the row's bytes");
+    if (!fill_strides(c->key_stride, c->key_bytes, batch, c->heads, c->capacity, p.kb, p.kh, p.ks) ||
+        !fill_strides(c->value_stride, c->value_bytes, batch, c->heads, c->capacity, p.vb, p.vh, p.vs))
+        return fail(ST_BAD_ARG, "cache strides let rows overlap, or span more than 2^56 bytes");
     if (!aligned_to(weights, type_bytes(c->type)) || !aligned_to(lens, 4) || !aligned_to(seen, 4) ||
         !aligned_to(rows, 4) || !aligned_to(acc, 4) || !aligned_to(pos, 4) || !aligned_to(out_acc, 4) ||
         !aligned_to(out_pos, 4) || !aligned_to(out_lens, 4))

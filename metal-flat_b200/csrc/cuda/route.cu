@@ -65,14 +65,13 @@ struct RouteParams {
 
 // Bounds of the errors of the two fp32 scores on the sides of a gap.  sigmoid = 1 / (1 + e):
 // e is off by 2^-22 + |x| 2^-23 of itself, which reaches s times 1 - s (below 8e-8),
-// 1 + e rounds (6e-8), the division is off by 2 ulp (1.2e-7).  softmax = e / sum: relative
-// errors of e (3e-7 at distances that matter), of the sum (3e-7 and |x - m| 2^-23
-// weighted by the terms, at most ln 1024 + 1 on average: 1e-6; a chain of at most 31
-// additions a lane weighted likewise, 5 levels: 7e-7 for 8 experts a lane, 2.2e-6 for
-// 32) and of the division, all of a score of at most the row's largest.  Adding the
-// bias rounds once more, 6e-8 of the result.
+// 1 + e rounds (6e-8), the reciprocal is off by 2^-23.  softmax = e / sum, in parts of
+// the row's largest score: e 2.9e-7; the sum 2.4e-7 and, |x - m| weighted by the terms
+// averaging at most ln 1024 + 1, 1.1e-6, its additions 2^-24 each for a lane's experts
+// and 5 levels; reciprocal and product 1.8e-7.  Adding the bias rounds once more, 6e-8
+// of the result.
 __device__ __forceinline__ float tau_base(bool softmax, float largest, int per_lane) {
-    return softmax ? 2.0f * (1.9e-6f + 6e-8f * per_lane) * largest + 2e-7f * largest : 5.4e-7f;
+    return softmax ? 2.0f * (2.3e-6f + 6e-8f * per_lane) * largest : 5.4e-7f;
 }
 __device__ __forceinline__ float tau_of(float base, float c) { return base + 1.3e-7f * fabsf(c); }
 
@@ -373,7 +372,7 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
     float a = none, b = none;
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-        const float v = c[j];       // -inf where there is no choice; NaN passes by
+        const float v = c[j];       // -inf where there is no choice
         b = fmaxf(b, fminf(a, v));
         a = fmaxf(a, v);
     }
@@ -499,7 +498,8 @@ __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* ro
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
         sh.keys[j * 32 + lane] = key[j];
-        if (key[j] >= floor_v && key[j] > neg_inf()) mine_bits |= 1u << j;
+        // (a floor of NaN, from infinite biases, lets all pass)
+        if (!(key[j] < floor_v) && key[j] > neg_inf()) mine_bits |= 1u << j;
     }
     const int count = __popc(mine_bits);
     int at = 0, n = 0;
@@ -635,8 +635,8 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
             base_tau = tau_base(p.softmax, largest, VPL);
 #pragma unroll
             for (int j = 0; j < VPL; ++j) {
-                // (a bias of NaN makes a key that no comparison takes)
-                c[j] = x[j] > neg_inf() ? c[j] + b[j] : neg_inf();
+                c[j] += b[j];
+                if (!(x[j] > neg_inf() && c[j] > neg_inf())) c[j] = neg_inf();     // a bias of NaN too
                 key[j] = p.bias ? c[j] : x[j];
             }
             if (p.groups > 1) doubt = choose_groups<LPT, VPL, false>(p, lane, c, base_tau, key);

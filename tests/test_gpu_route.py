@@ -133,6 +133,32 @@ def test_values_that_leave_little_or_nothing(kind, score):
         check(x, 5, score, b, renormalise=renorm, groups=6, kept=2, top=2)
 
 
+@pytest.mark.parametrize("n", [64, 200, 256, 512, 1024])
+def test_wide_rows_of_equals_and_of_strange_values(n):
+    """More equal logits than a warp ranks, and -inf, NaN and infinities among them."""
+    inf, nan = float("inf"), float("nan")
+    g = gen(("wide", n))
+    x = torch.zeros(12, n)
+    x[1] = 3.0
+    x[2] = torch.randint(0, 2, (n,), generator=g).float()
+    x[3, ::3] = -inf
+    x[4, 1::2] = nan
+    x[5, n // 2:] = -inf
+    x[6] = -inf
+    x[6, n - 1] = 1.0
+    x[7, 5], x[7, n - 2] = inf, inf
+    x[8:] = torch.randn(4, n, generator=g)
+    x[9, ::7] = nan
+    bias = 0.1 * torch.randn(n, generator=g)
+    bias[::5], bias[3], bias[n // 2] = nan, -inf, inf
+    x, bias = x.cuda(), bias.cuda()
+    for score, b in itertools.product(["softmax", "sigmoid"], [None, bias, torch.zeros(n).cuda()]):
+        for k in (1, 8, 32):
+            check(x, k, score, b, renormalise=k == 8)
+        for groups, kept, top in [(8, 3, 2), (8, 8, 1), (4, 1, 2)]:
+            check(x, 4, score, b, groups=groups, kept=kept, top=top)
+
+
 def test_far_logits_keep_their_quotients():
     """sigmoid scores that underflow fp32 still divide: weights from exponents."""
     x = torch.tensor([[-200.0, -201.0, -203.0, -400.0], [300.0, 250.0, -250.0, 0.0]]).cuda()

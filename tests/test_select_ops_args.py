@@ -84,7 +84,7 @@ def test_beam_specs(built_lib, bad):
 def test_beam_arguments(built_lib):
     b = M.BeamSearch(4, 1000, 8, dtype="fp16")
     need = b.workspace_bytes(3)
-    ok = dict(logits=P, cum=P, batch=3, parents=P, tokens=P, scores=P, ws=P, ws_bytes=need)
+    ok = dict(logits=P, cum=P, batch=3, parents=P, tokens=P, scores=2 * P, ws=P, ws_bytes=need)
     for name in ("logits", "cum", "parents", "tokens", "scores"):
         assert status(b.select_device, **{**ok, name: 0}) == NULL
         assert status(b.select_device, **{**ok, name: P + 1}) == BAD
@@ -92,6 +92,7 @@ def test_beam_arguments(built_lib):
     assert status(b.select_device, **{**ok, "batch": 2 ** 30, "ws_bytes": 1 << 62}) == BAD
     assert status(b.select_device, **{**ok, "stride": 999}) == BAD
     assert status(b.select_device, **{**ok, "finished": P}) == BAD      # finished beams without an eos
+    assert status(b.select_device, **{**ok, "scores": P, "cum": P}) == BAD      # over the cums, with k != beams
     if need:
         assert status(b.select_device, **{**ok, "ws": 0}) == BAD
         assert status(b.select_device, **{**ok, "ws": P + 8}) == BAD
@@ -115,7 +116,7 @@ def test_reorder_arguments(built_lib):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(heads=0), dict(group=0), dict(capacity=0), dict(budget=0), dict(budget=101), dict(recent=-1), dict(sink=-1),
+    dict(heads=0), dict(group=0), dict(capacity=0), dict(capacity=2 ** 30 + 1), dict(budget=0), dict(budget=101), dict(recent=-1), dict(sink=-1),
     dict(recent=30, sink=21), dict(recent=2 ** 31 - 1, sink=2 ** 31 - 1), dict(dtype=5), dict(key_bytes=-1),
     dict(value_bytes=-16)])
 def test_cache_specs(built_lib, bad):
@@ -139,12 +140,14 @@ def test_cache_arguments(built_lib):
     assert status(c.evict_device, **{**ok, "batch": -1}) == BAD
     assert status(c.evict_device, **{**ok, "batch": 40_000, "ws_bytes": 1 << 62}) == BAD
     assert status(c.evict_device, **{**ok, "queries": -1}) == BAD
+    assert status(c.evict_device, **{**ok, "queries": 2 ** 30}) == BAD
     assert status(c.evict_device, **{**ok, "weight_stride": (1, 1, -1)}) == BAD
     if need:
         assert status(c.evict_device, **{**ok, "ws": 0}) == BAD
         assert status(c.evict_device, **{**ok, "ws": P + 4}) == BAD
         assert status(c.evict_device, **{**ok, "ws_bytes": need - 1}) == BAD
-    for stride in [(3200, 1600, 15), (3200, 15, 16), (15, 1600, 16), (-3200, 1600, 16), (0, 1600, 16)]:
+    for stride in [(3200, 1600, 15), (3200, 15, 16), (15, 1600, 16), (-3200, 1600, 16), (0, 1600, 16), (3199, 1600, 16),
+                   (3200, 1599, 16), (3200, 16, 31), (1 << 62, 1600, 16)]:
         short = M.CacheEviction(2, 4, 100, 50, 16, 16, key_stride=stride)
         assert status(short.evict_device, **ok) == BAD, stride
         short = M.CacheEviction(2, 4, 100, 50, 16, 16, value_stride=stride)
