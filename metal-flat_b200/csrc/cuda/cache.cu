@@ -11,6 +11,12 @@
 // One kernel does it all: a cluster of 1 to 8 blocks owns a (sequence, head), keeps
 // its sums and keys in shared memory and exchanges histograms and counts there.
 // The three kernels behind it are for caches longer than eight blocks hold.
+//
+// 32 x 8 caches of 4097 slots and 4 weights each, one entry leaving (25 MB, 3.9 us at the
+// copy rate): 15.4 us, of which 8 sum up and the rest are the exchanges of the select.
+// 4 x 8 prompts of up to 16,384 slots and 64 rows cut to 1024 (84 MB, 13 us): 38 us,
+// 17 for the sums (two-sums of packed floats), 9 for the select, 5 for lists and 5 for
+// the rows.  Three kernels over global memory took 69 and 155.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -14,6 +14,12 @@
 // kernel sums the counts of the tiles before and scatters.  Nothing depends on
 // the order in which blocks run.  Up to kClusterTokens tokens the tiles' blocks are one
 // cluster, which exchanges the counts in shared memory and scatters by itself.
+//
+// Bound by instructions: 16,384 tokens x 256 experts in 8 groups with a bias (16.8 MB,
+// 2.9 us at the copy rate) take 31.5 us, 25 of them in route_kernel at 0.7 instructions a
+// clock and scheduler; of a token's 925 instructions 265 load it and weigh its choice,
+// 95 find the floor, 135 list what reaches it, 135 rank that, 110 form the scores and 180
+// choose groups.  64 tokens take 8.9 us.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -831,7 +837,9 @@ __global__ void __launch_bounds__(kListThreads) lists_kernel(const __grid_consta
 // Gradient of the logits, LPT lanes per token as in the forward pass.  With w =
 // scale * s (s a softmax p): dx_e = scale * p_e (g_e - sum_j g_j p_j); sigmoid:
 // dx_e = scale * g_e s_e (1 - s_e).  Renormalised over the chosen (w = scale * s /
-// S): dx_j = w_j (g_j - sum_i g_i w_i / scale), for a sigmoid times 1 - s_j.
+// S): dx_j = w_j (g_j - sum_i g_i w_i / scale), for a sigmoid times 1 - s_j.  32,768 x 128
+// bf16 take 8.8 us (16.8 MB: 1.9 TB/s), bound by instructions; with 4 experts a lane and
+// one token a warp they took 17.6.
 template <class T, int LPT, int VPL>
 __global__ void __launch_bounds__(kGradThreads)
     route_backward_kernel(const RouteParams p, const float* __restrict__ grad, T* out,
