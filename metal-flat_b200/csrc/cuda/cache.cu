@@ -13,7 +13,7 @@
 // The three kernels behind it are for caches longer than eight blocks hold.
 //
 // 32 x 8 caches of 4097 slots and 4 weights each, one entry leaving (25 MB, 3.9 us at the
-// copy rate): 15.4 us, of which 8 sum up and the rest are the exchanges of the select.
+// copy rate): 14.4 us, of which 7 sum up and the rest are the exchanges of the select.
 // 4 x 8 prompts of up to 16,384 slots and 64 rows cut to 1024 (84 MB, 13 us): 38 us,
 // 17 for the sums (two-sums of packed floats), 9 for the select, 5 for lists and 5 for
 // the rows.  Three kernels over global memory took 69 and 155.
@@ -175,19 +175,28 @@ struct TwoFloats2 {
     }
 };
 
-// a[i] plus the weights of four adjacent slots over all rows (`rows` query rows of
-// each of the group's heads), kAtOnce rows in flight; w is aligned for four.
-template <int kAtOnce, class T>
-__device__ __forceinline__ void add_rows(const T* w, int64_t wh, int64_t wq, int group, int rows, float (&a)[4]) {
+// a[i] plus the weights of four slots over all rows (`rows` query rows of each of the
+// group's heads), kAtOnce rows in flight.  kVec: four adjacent slots, w aligned for them;
+// else the first `most` of w[0], w[kEvictThreads], ...
+template <int kAtOnce, bool kVec, class T>
+__device__ __forceinline__ void add_rows(const T* w, int64_t wh, int64_t wq, int group, int rows, int most,
+                                         float (&a)[4]) {
     TwoFloats2 s0{make_float2(a[0], a[1]), make_float2(0.0f, 0.0f)}, s1{make_float2(a[2], a[3]), make_float2(0.0f, 0.0f)};
     const int64_t back = wh - static_cast<int64_t>(rows - 1) * wq;      // to the next head's first row
     const int all = group * rows;
     for (int i = 0, r = 0; i < all; i += kAtOnce) {
         Pack<T, 4> v[kAtOnce];
+        T one[kAtOnce][4];
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-            v[u].raw = {};
-            if (i + u < all) v[u].load(w);
+            if constexpr (kVec) {
+                v[u].raw = {};
+                if (i + u < all) v[u].load(w);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    one[u][c] = i + u < all && c < most ? w[c * kEvictThreads] : from_float<T>(0.0f);
+            }
             const bool last = ++r == rows;
             w += last ? back : wq;
             r = last ? 0 : r;
@@ -195,7 +204,12 @@ __device__ __forceinline__ void add_rows(const T* w, int64_t wh, int64_t wq, int
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
             float x[4];
-            v[u].unpack(x);
+            if constexpr (kVec) {
+                v[u].unpack(x);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] = to_float(one[u][c]);
+            }
             s0.add(make_float2(x[0], x[1]));
             s1.add(make_float2(x[2], x[3]));
         }
@@ -266,8 +280,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
             keys[j] = slot_key(p, a, q, since);
         }
     };
-    // whole fours, a thread each; then the slots behind them, or all where the weights
-    // are not aligned for it
+    // aligned weights: whole fours, a thread each
     const int fours = p.vec_w ? mine & ~3 : 0;
     for (int j = threadIdx.x * 4; j < fours; j += kEvictThreads * 4) {
         float a[4];
@@ -285,8 +298,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
             }
         }
         // (a token's few rows, or a prompt's many: 16 in flight took 37.4 us where 8 took 39.3)
-        if (p.group * rows > 4) add_rows<16>(weights + j, p.wh, p.wq, p.group, rows, a);
-        else if (rows > 0) add_rows<4>(weights + j, p.wh, p.wq, p.group, rows, a);
+        if (p.group * rows > 4) add_rows<16, true>(weights + j, p.wh, p.wq, p.group, rows, 4, a);
+        else if (rows > 0) add_rows<4, true>(weights + j, p.wh, p.wq, p.group, rows, 4, a);
         if (p.vec_a && (lo + j + 4 <= m || lo + j >= m)) {
             if (lo + j < m) {
                 *reinterpret_cast<float4*>(out_acc + lo + j) = make_float4(a[0], a[1], a[2], a[3]);
@@ -303,20 +316,26 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
             for (int i = 0; i < 4; ++i) put(j + i, a[i], q[i]);
         }
     }
-    if (p.group * rows < 16 || fours == 0) {
-        // (few rows, or many slots: a thread each)
-        for (int j = fours + threadIdx.x; j < mine; j += kEvictThreads) {
-            TwoFloats s{acc[j], 0.0f};
-            const T* w = weights + j;
-            for (int g = 0; g < p.group && rows > 0; ++g)
-#pragma unroll 8
-                for (int r = 0; r < rows; ++r) s.add(to_float(w[g * p.wh + r * p.wq]));
-            put(j, s.rounded(), pos[j]);
-        }
-    } else {
-        for (int j = fours + static_cast<int>(threadIdx.x >> 5); j < mine; j += kEvictWarps) {
+    if (p.vec_w) {                      // at most three slots are left: a warp each
+        const int j = fours + static_cast<int>(threadIdx.x >> 5);
+        if (j < mine) {
             const float a = add_rows_warp(weights + j, p.wh, p.wq, p.group, rows, acc[j]);
             if ((threadIdx.x & 31) == 0) put(j, a, pos[j]);
+        }
+    } else {                            // rows at odd places: neighbouring threads, neighbouring slots
+        for (int j = threadIdx.x; j < mine; j += kEvictThreads * 4) {
+            const int most = (mine - j + kEvictThreads - 1) / kEvictThreads;
+            float a[4];
+            int q[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                a[c] = c < most ? acc[j + c * kEvictThreads] : 0.0f;
+                q[c] = c < most ? pos[j + c * kEvictThreads] : 0;
+            }
+            if (rows > 0) add_rows<4, false>(weights + j, p.wh, p.wq, p.group, rows, most, a);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < most) put(j + c * kEvictThreads, a[c], q[c]);
         }
     }
     if (!over) return;
@@ -472,7 +491,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     float* tail_acc = p.tail_acc + bh * p.half;
     int32_t* tail_pos = p.tail_pos + bh * p.half;
     tie = tie0;
-    for (int j = j0; j < j1; ++j) {
+    for (int j = moved ? j0 : j1; j < j1; ++j) {        // most runs have nothing to list
         const uint32_t key = keys[j];
         const bool keep = key > cut || (key == cut && tie++ < ties);
         if (lo + j < m) {
