@@ -416,7 +416,7 @@ class Router:
                                int(bool(renormalise)), int(groups), int(groups_kept),
                                int(group_top), float(scale))
         self.device = int(device)
-        self._ref = ctypes.addressof(self.spec)
+        self._ref = ctypes.byref(self.spec)
         self._lib = lib()
 
     def workspace_bytes(self, tokens: int) -> int:
@@ -451,7 +451,7 @@ class BeamSearch:
                  device: int = -1):
         self.spec = BeamSpec(int(beams), int(vocab), int(k), _code(STORAGES, dtype), int(eos))
         self.device = int(device)
-        self._ref = ctypes.addressof(self.spec)
+        self._ref = ctypes.byref(self.spec)
         self._lib = lib()
 
     def workspace_bytes(self, batch: int) -> int:
@@ -493,7 +493,7 @@ class CacheEviction:
                               int(sink), _code(STORAGES, dtype), int(key_bytes), int(value_bytes),
                               three(*key_stride), three(*value_stride))
         self.device = int(device)
-        self._ref = ctypes.addressof(self.spec)
+        self._ref = ctypes.byref(self.spec)
         self._lib = lib()
 
     def workspace_bytes(self, batch: int) -> int:

@@ -62,6 +62,7 @@ SIZES = [  # batch, beams, vocab, k
     (1, 1, 1, 1), (2, 1, 3, 2), (1, 2, 1, 4), (3, 3, 7, 6), (2, 4, 31, 9), (1, 4, 257, 8), (5, 5, 1000, 10),
     (2, 8, 4099, 16), (1, 16, 8191, 32), (1, 64, 300, 128), (1, 33, 2049, 66), (3, 2, 32000, 4), (1, 3, 50257, 128),
     (2, 1, 128_000, 100), (1, 2, 70_001, 1), (1, 1, 262_147, 2), (7, 6, 511, 12),
+    (700, 3, 37, 4), (40, 8, 6007, 16),
 ]
 
 

@@ -89,6 +89,7 @@ SIZES = [  # batch, heads, group, queries, capacity, lens, budget, recent, sink
     (1, 3, 2, 1, 1025, [1025], 1024, 0, 1), (2, 2, 1, 7, 2000, [2000, 1500], 37, 10, 4),
     (1, 2, 3, 5, 4099, [4098], 4000, 100, 0), (1, 1, 1, 1, 9000, [9000], 1, 0, 0), (1, 2, 2, 2, 8193, [8000], 4096, 0, 0),
     (3, 8, 4, 1, 130, [129, 130, 128], 128, 16, 4),
+    (150, 8, 2, 1, 41, [(7 * i) % 42 for i in range(150)], 20, 5, 1),
 ]
 
 
@@ -198,6 +199,18 @@ def test_weights_with_strides(kind):
         assert torch.equal(a, b)
 
 
+def test_weights_shared_by_all_heads():
+    """A stride of 0: one row of weights for every query head."""
+    g = gen("shared")
+    for cap in (60, 61):
+        data = make(g, 2, 2, cap, [cap, 50])
+        w = torch.rand(2, 1, 1, cap, generator=g)
+        want = check([cap, 50], [cap, 50], *data, 30, 0, 0, w.expand(2, 6, 1, cap).contiguous(), 3)
+        got = run([cap, 50], [cap, 50], *data, 30, weights=w, group=3, queries=1, weight_stride=(cap, 0, 0))
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+
+
 def test_a_value_buffer_alone_and_none():
     g = gen("values only")
     acc, pos, keys, values = make(g, 1, 2, 60, [60])
@@ -216,7 +229,7 @@ def test_a_value_buffer_alone_and_none():
             assert torch.equal(v.cpu()[0, j, :20], values[0, j, at if vb else slice(0, 20)])
 
 
-@pytest.mark.parametrize("cap", [40_000, 150_001, 196_609, 300_003])
+@pytest.mark.parametrize("cap", [40_000, 150_001, 196_608, 196_609, 300_003])
 def test_long_caches(cap):
     g = gen(("long", cap))
     acc, pos, keys, values = make(g, 1, 2, cap, [cap - 3], dim=2)

@@ -192,6 +192,26 @@ def test_many_tokens_and_lists():
     check(x, 4, "sigmoid")
 
 
+def test_more_tokens_than_16_bit_counts_hold():
+    """Tiles are cut at 65,535 tokens; one expert takes nearly all of them."""
+    t, n = 9_800_000, 3
+    x = torch.zeros(t, n, device="cuda")
+    x[:, 1] = 1.0
+    x[::1000, 2] = 2.0
+    r = M.Router(n, 1)
+    ids = torch.empty(t, 1, dtype=torch.int32, device="cuda")
+    w = torch.empty(t, 1, device="cuda")
+    start = torch.empty(n + 1, dtype=torch.int32, device="cuda")
+    slots = torch.empty(t, dtype=torch.int32, device="cuda")
+    ws = torch.empty(r.workspace_bytes(t), dtype=torch.uint8, device="cuda")
+    r.route_device(x.data_ptr(), t, ids.data_ptr(), w.data_ptr(), start=start.data_ptr(), slots=slots.data_ptr(),
+                   ws=ws.data_ptr(), ws_bytes=ws.numel())
+    want = x.argmax(1)
+    assert torch.equal(ids[:, 0].long(), want)
+    assert start.tolist() == [0, 0, t - t // 1000, t]
+    assert torch.equal(slots.long(), torch.sort(want, stable=True).indices)
+
+
 def test_no_tokens_gives_empty_lists():
     r = M.Router(10, 2)
     start = torch.full((11,), 5, dtype=torch.int32, device="cuda")
