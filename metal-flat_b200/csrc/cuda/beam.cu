@@ -564,13 +564,19 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         else if (x == -neg_inf()) c.key = choice_key(base);
         return c;
     };
-    // fn(choice) for every candidate of the thread
-    auto each = [&](auto&& fn) {
+    Choice own[kHeld];          // the held ones' keys, formed once an attempt
+    auto form = [&] {
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
             const int i = j * kRowThreads + first;
-            if (i < total) fn(choice_of(i, held[j]));
+            own[j] = i < total ? choice_of(i, held[j]) : Choice{0, 0};
         }
+    };
+    // fn(choice) for every candidate of the thread
+    auto each = [&](auto&& fn) {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (own[j].key != 0) fn(own[j]);
         for (int i = kHeld * kRowThreads + first; i < total; i += kRowThreads) fn(choice_of(i, cand[i]));
     };
     for (int attempt = 0; ; ++attempt) {
@@ -584,6 +590,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
                 sh_err = 2.0f * e;
             }
         }
+        form();
         uint64_t mine = 0;
         each([&](const Choice& c) { mine = c.key > mine ? c.key : mine; });
         // a floor in fp32, rounded down, and lower by the sums' error: a key that much
