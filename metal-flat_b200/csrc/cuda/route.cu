@@ -89,18 +89,14 @@ __device__ __forceinline__ float exp_of<float>(float v) { return exp2_fast(v * k
 template <>
 __device__ __forceinline__ double exp_of<double>(double v) { return exp(v); }
 
-template <int LPT, class V>
-__device__ __forceinline__ V lane_max(V v) {
-    if constexpr (LPT == 32 && sizeof(V) == 4) {
-        return __reduce_max_sync(kFullMask, v);
-    } else {
+template <int LPT>
+__device__ __forceinline__ uint64_t lane_max(uint64_t v) {
 #pragma unroll
-        for (int o = LPT / 2; o > 0; o >>= 1) {
-            const V w = __shfl_xor_sync(kFullMask, v, o);
-            v = w > v ? w : v;
-        }
-        return v;
+    for (int o = LPT / 2; o > 0; o >>= 1) {
+        const uint64_t w = __shfl_xor_sync(kFullMask, v, o);
+        v = w > v ? w : v;
     }
+    return v;
 }
 
 template <int LPT, class S>
@@ -110,8 +106,6 @@ __device__ __forceinline__ S lane_sum(S v) {
     return v;
 }
 
-// Scores of the lane's experts, lane l of a token holding experts
-// [l * VPL, (l + 1) * VPL).  x: fp32 logits, -inf for "none".
 // e[j] = exp(x[j] - m), m the row's largest: 0 for -inf, and where m itself is infinite 1
 // for the logits that are m.  Returns the lane's sum.
 template <class S, int VPL>
@@ -138,6 +132,8 @@ __device__ __forceinline__ S inverse(S v) {
     if constexpr (sizeof(S) == 4) return inverse_fast(v);
     else return S(1) / v;
 }
+// Scores of the lane's experts, lane l of a token holding experts [l * VPL, (l + 1) * VPL),
+// and a bound of the row's largest.  x: fp32 logits, -inf for "none".
 template <class S, int LPT, int VPL>
 __device__ __forceinline__ void scores_of(const float (&x)[VPL], bool softmax, S (&s)[VPL], S& largest) {
     largest = S(1);
@@ -207,21 +203,21 @@ __device__ __forceinline__ unsigned kept_groups(const RouteParams& p, int lane, 
 
 // The k largest keys, ties to the lowest expert: lane r of the token gets the
 // r-th expert (or -1) and its logit.
-template <int LPT, int VPL, class K>
-__device__ __forceinline__ void take_best(K (&key)[VPL], const float (&x)[VPL], int k, int lane,
+template <int LPT, int VPL>
+__device__ __forceinline__ void take_best(uint64_t (&key)[VPL], const float (&x)[VPL], int k, int lane,
                                           int& id, float& xid) {
     const int base = (threadIdx.x & 31) - lane;
     id = -1;
     xid = neg_inf();
     for (int r = 0; r < k; ++r) {
-        K best = 0;
+        uint64_t best = 0;
         int at = 0;
         float xb = 0.0f;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
             if (key[j] > best) { best = key[j]; at = j; xb = x[j]; }
         }
-        const K top = lane_max<LPT>(best);
+        const uint64_t top = lane_max<LPT>(best);
         const unsigned who = __ballot_sync(kFullMask, best == top) >> base;
         const int src = __ffs(who) - 1;
         const int e = __shfl_sync(kFullMask, lane * VPL + at, base + src);
@@ -564,8 +560,8 @@ __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* ro
     return false;
 }
 
-// Exclusive sums of one value per thread's run over the block's values v[0, n) in
-// shared memory, in place; returns nothing.  n <= 1024.
+// Exclusive sums of v[0, n) in shared memory, in place: a thread sums a run, the runs'
+// sums are scanned over the block.
 template <int NT>
 __device__ __forceinline__ void block_exclusive(int* v, int n, int* warp_sum) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -690,7 +686,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
     if (!p.start) return;
 
     // ranks: warps own adjacent runs of the tile's choices
-    __shared__ uint16_t hist[kWarps][kMost];
+    __shared__ __align__(16) uint16_t hist[kWarps][kMost];      // cleared by words
     __shared__ int total[kMost + 1], before[kMost];
     __shared__ int warp_sum[32];
     const int full_lane = threadIdx.x & 31;
