@@ -6,7 +6,8 @@
 // is exact.  With a bias the order is that of c in 64 bits: the kernel forms c in
 // fp32, whose error is below tau, and takes the selection when every gap between
 // neighbours in it (and at the cut between kept and dropped groups) exceeds
-// tau; the other tokens are selected again from scores in 64 bits.
+// tau; a closer cut, and the few candidates of a closer selection, are settled by scores
+// in 64 bits.
 //
 // Lists.  The tokens are cut into tiles, one block each.  A block ranks its choices
 // among those of the same expert in its tile (in order: warps own adjacent choices
@@ -293,63 +294,96 @@ __device__ __forceinline__ void load_row(const RouteParams& p, int64_t t, int la
         if (!(x[j] > neg_inf())) x[j] = neg_inf();
 }
 
-// A token from scores in 64 bits, for any values: the row is read again, so that the
-// common path keeps its registers.  Every lane of the warp calls it.
+// A token's choice keys in 64 bits (0: no choice), from the row read again.
 template <class T, int LPT, int VPL>
-__device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int lane, bool live,
-                                         int& id, float& xid) {
+__device__ __forceinline__ void exact_keys(const RouteParams& p, const float (&x)[VPL], int lane,
+                                           double (&c)[VPL], uint64_t (&key)[VPL]) {
+    if (p.bias || (p.groups > 1 && p.group_top == 2)) {
+        double largest;
+        scores_of<double, LPT, VPL>(x, p.softmax, c, largest);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) c[j] = x[j];
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        const int e = lane * VPL + j;
+        if (p.bias && e < p.experts) c[j] += static_cast<double>(p.bias[e]);
+        key[j] = x[j] == neg_inf() ? 0ull : choice_key(p.bias ? c[j] : static_cast<double>(x[j]));
+    }
+}
+
+// A token's kept groups in 64 bits, as bits; where a group is 2^n lanes, all bits of its
+// lanes alike.  The row is read again, so that the common path keeps its registers.
+// Every lane of the warp calls it.
+template <class T, int LPT, int VPL>
+__device__ __noinline__ unsigned exact_groups(const RouteParams& p, int64_t t, int lane, bool live) {
     float x[VPL];
     load_row<T, LPT, VPL>(p, t, lane, live, x);
     uint64_t key[VPL];
-    if (p.bias || (p.groups > 1 && p.group_top == 2)) {
-        double c[VPL];
+    double c[VPL];
+    exact_keys<T, LPT, VPL>(p, x, lane, c, key);
+    if (p.lane_groups == 0) {
         bool in[VPL];
-        double largest;
-        scores_of<double, LPT, VPL>(x, p.softmax, c, largest);
+        float unused;
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            const int e = lane * VPL + j;
-            if (p.bias && e < p.experts) c[j] += static_cast<double>(p.bias[e]);
-            key[j] = x[j] == neg_inf() ? 0ull : choice_key(p.bias ? c[j] : static_cast<double>(x[j]));
-            in[j] = key[j] != 0;
-        }
-        if (p.groups > 1) {
-            float unused;
-            const unsigned kept = kept_groups<double, LPT>(
-                p, lane, group_scores<double, LPT, VPL>(p, lane, c, in, 0.0f, unused));
-            const int size = p.experts / p.groups;
+        for (int j = 0; j < VPL; ++j) in[j] = key[j] != 0;
+        return kept_groups<double, LPT>(p, lane, group_scores<double, LPT, VPL>(p, lane, c, in, 0.0f, unused));
+    }
+    const double none = static_cast<double>(neg_inf());
+    double a = none, b = none;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (!((kept >> min((lane * VPL + j) / size, 31)) & 1u)) key[j] = 0;
-        }
-    } else {
-        bool in[VPL];
+    for (int j = 0; j < VPL; ++j) {
+        const double v = key[j] != 0 ? c[j] : none;
+        b = fmax(b, fmin(a, v));
+        a = fmax(a, v);
+    }
+    for (int o = 1; o < p.lane_groups; o <<= 1) {
+        const double a2 = __shfl_xor_sync(kFullMask, a, o), b2 = __shfl_xor_sync(kFullMask, b, o);
+        b = fmax(fmin(a, a2), fmax(b, b2));
+        a = fmax(a, a2);
+    }
+    const double mine = p.group_top == 2 && b > none ? a + b : a;
+    const int base = (threadIdx.x & 31) - lane, group = lane / p.lane_groups;
+    int above = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        const double v = __shfl_sync(kFullMask, mine, base + g * p.lane_groups);
+        above += v > mine || (v == mine && g < group) ? 1 : 0;
+    }
+    return group < p.groups && above < p.groups_kept ? ~0u : 0u;
+}
+
+// Whether an expert's group is among those that exact_groups() keeps.
+__device__ __forceinline__ bool group_kept(const RouteParams& p, unsigned kept, int expert) {
+    return p.lane_groups ? kept != 0u : ((kept >> min(expert / (p.experts / p.groups), 31)) & 1u) != 0u;
+}
+
+// A token from scores in 64 bits, for any values.  Every lane of the warp calls it.
+template <class T, int LPT, int VPL>
+__device__ __noinline__ void exact_token(const RouteParams& p, int64_t t, int lane, bool live,
+                                         int& id, float& xid) {
+    const unsigned kept = p.groups > 1 ? exact_groups<T, LPT, VPL>(p, t, lane, live) : 0u;
+    float x[VPL];
+    load_row<T, LPT, VPL>(p, t, lane, live, x);
+    uint64_t key[VPL];
+    double c[VPL];
+    exact_keys<T, LPT, VPL>(p, x, lane, c, key);
+    if (p.groups > 1) {
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-            key[j] = choice_key(static_cast<double>(x[j]));
-            in[j] = key[j] != 0;
-        }
-        if (p.groups > 1) {
-            float unused;
-            const unsigned kept = kept_groups<float, LPT>(
-                p, lane, group_scores<float, LPT, VPL>(p, lane, x, in, 0.0f, unused));
-            const int size = p.experts / p.groups;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (!((kept >> min((lane * VPL + j) / size, 31)) & 1u)) key[j] = 0;
-        }
+        for (int j = 0; j < VPL; ++j)
+            if (!group_kept(p, kept, lane * VPL + j)) key[j] = 0;
     }
     take_best<LPT, VPL>(key, x, p.k, lane, id, xid);
 }
 
-// The groups' part of the choice in fp32: -inf for experts outside the kept ones.
+// The groups' part of the choice in fp32: `bits` as exact_groups() gives them.
 // Returns whether the cut is too close for fp32 (exact: c are logits, no doubt but
 // ties, which go to the lower group).  Where a group is 2^n lanes of a warp, their
 // top two meet in n exchanges, and each group is compared with all others: kept for
 // sure, dropped for sure, or in doubt.
 template <int LPT, int VPL, bool exact>
 __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, const float (&c)[VPL],
-                                              float base_tau, float (&key)[VPL]) {
+                                              float base_tau, const float (&key)[VPL], unsigned& bits) {
     const float none = neg_inf();
     if (p.lane_groups == 0) {
         bool in[VPL];
@@ -357,18 +391,14 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
 #pragma unroll
         for (int j = 0; j < VPL; ++j) in[j] = key[j] > none;
         const float mine = group_scores<float, LPT, VPL>(p, lane, c, in, base_tau, tau);
-        const unsigned kept = kept_groups<float, LPT>(p, lane, mine);
-        const int size = p.experts / p.groups;
-        const bool here = lane < p.groups && ((kept >> lane) & 1u);
+        bits = kept_groups<float, LPT>(p, lane, mine);
+        const bool here = lane < p.groups && ((bits >> lane) & 1u);
         float low = here ? mine : -none, cut = lane < p.groups && !here ? mine : none;
 #pragma unroll
         for (int o = LPT / 2; o > 0; o >>= 1) {
             low = fminf(low, __shfl_xor_sync(kFullMask, low, o));
             cut = fmaxf(cut, __shfl_xor_sync(kFullMask, cut, o));
         }
-#pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            if (!((kept >> min((lane * VPL + j) / size, 31)) & 1u)) key[j] = none;
         return !exact && cut > none && !(low - cut > tau);
     }
     float a = none, b = none;
@@ -409,10 +439,7 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
     const int above = counts & 0xffff, near = counts >> 16;
     const bool kept = exact ? above < p.groups_kept : near <= p.groups_kept;
     const bool dropped = above >= p.groups_kept || mine == none;
-    if (!kept) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) key[j] = none;
-    }
+    bits = kept ? ~0u : 0u;
     return group < p.groups && !kept && !dropped;
 }
 
@@ -544,6 +571,7 @@ __device__ __forceinline__ bool take_best_warp(const RouteParams& p, const T* ro
             id = -1;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                if (32 * h >= n) break;
                 const int e = lane + 32 * h < n ? __float_as_int(sh.cand[lane + 32 * h].y) : 0;
                 int rank = 0;
                 for (int m = 0; m < n; ++m) {
@@ -631,6 +659,7 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
         }
         bool doubt = false;
         float base_tau = 0.0f;
+        unsigned kept = 0;
         if (by_sums) {
             float c[VPL], largest;
             scores_of<float, LPT, VPL>(x, p.softmax, c, largest);
@@ -641,11 +670,17 @@ __global__ void __launch_bounds__(NT) route_kernel(const __grid_constant__ Route
                 if (!(x[j] > neg_inf() && c[j] > neg_inf())) c[j] = neg_inf();     // a bias of NaN too
                 key[j] = p.bias ? c[j] : x[j];
             }
-            if (p.groups > 1) doubt = choose_groups<LPT, VPL, false>(p, lane, c, base_tau, key);
+            if (p.groups > 1 && __any_sync(kFullMask, choose_groups<LPT, VPL, false>(p, lane, c, base_tau, key, kept)))
+                kept = exact_groups<T, LPT, VPL>(p, t, lane, live);
         } else {
 #pragma unroll
             for (int j = 0; j < VPL; ++j) key[j] = x[j];
-            if (p.groups > 1) choose_groups<LPT, VPL, true>(p, lane, x, 0.0f, key);
+            if (p.groups > 1) choose_groups<LPT, VPL, true>(p, lane, x, 0.0f, key, kept);
+        }
+        if (p.groups > 1) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (!group_kept(p, kept, lane * VPL + j)) key[j] = neg_inf();
         }
         int id = -1;
         float xid = neg_inf();
