@@ -9,8 +9,10 @@
 // order.
 //
 // One kernel does it all: a cluster of 1 to 8 blocks owns a (sequence, head), keeps
-// its sums and keys in shared memory and exchanges histograms and counts there.
-// The three kernels behind it are for caches longer than eight blocks hold.
+// its sums and keys in shared memory and exchanges histograms and counts there.  Above
+// 196,608 slots a head the sums wait in the workspace (250,001 slots, 2 heads, 48,000 moves
+// each: 212 us, against 1.4 ms by the three kernels behind it); those three are for
+// caches of more than 393,216 slots, whose keys eight blocks cannot hold.
 //
 // 32 x 8 caches of 4097 slots and 4 weights each, one entry leaving (25 MB, 3.9 us at the
 // copy rate): 14.4 us, of which 7 sum up and the rest are the exchanges of the select.
@@ -30,7 +32,7 @@ namespace mflat_cu {
 namespace {
 
 constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
-constexpr int kEvictSlots = 24576;      // slots a block holds, 8 bytes each
+constexpr int kEvictSlots = 49152;      // keys a block holds, 4 bytes each; with half as many, sums too
 constexpr int kEvictCluster = 8;
 constexpr int kMaxCapacity = 1 << 30;
 constexpr int kGather = 2048;           // keys of one digit that a block takes in
@@ -57,7 +59,8 @@ struct CacheParams {
     int vec_w, vec_a;                   // weights, and acc and pos, can be moved by fours
     int range;                          // slots that a block of evict_kernel has room for
     int half;                           // most moves of a head: capacity / 2
-    float* sums;                        // long caches [b][h][capacity]: acc'
+    int64_t sums_row;                   // capacity rounded up to 4
+    float* sums;                        // long caches [b][h][sums_row]: acc' (null: in shared memory)
     int32_t* holes;                     // workspace [b][h][half]
     int32_t* tails;                     // workspace [b][h][half]: slot,
     float* tail_acc;                    // acc' and
@@ -250,7 +253,6 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     __shared__ __align__(16) int small[128];
     __shared__ int sh_left, sh_share, sh_own, sh_ties, sh_moves;
     uint32_t* keys = dyn;
-    float* sums = reinterpret_cast<float*>(dyn + p.range);
     const int64_t bh = blockIdx.y;
     const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh % p.heads);
     const uint32_t me = blockIdx.x, blocks = gridDim.x;
@@ -259,6 +261,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     const int range = ((n + static_cast<int>(blocks) - 1) / static_cast<int>(blocks) + 3) & ~3;
     const int lo = static_cast<int>(me) * range;
     const int mine = max(0, min(range, n - lo));
+    float* sums = p.sums ? p.sums + bh * p.sums_row + lo : reinterpret_cast<float*>(dyn + p.range);
     const float* acc = p.acc + bh * p.capacity + lo;
     const int32_t* pos = p.pos + bh * p.capacity + lo;
     float* out_acc = p.out_acc + bh * p.capacity;
@@ -470,7 +473,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
         tie = INT_MIN / 2;
     }
     const int tie0 = tie;
-    int moved = 0;                      // holes in the upper half word, tails in the lower
+    // holes in the upper half word, tails in the lower: a block has fewer than 2^16 of each,
+    // so sums stay apart (as unsigned: 2^15 holes reach the sign)
+    static_assert(kEvictSlots < 65536, "counts in half words");
+    int moved = 0;
     for (int j = j0; j < j1; ++j) {
         const uint32_t key = keys[j];
         const bool keep = key > cut || (key == cut && tie++ < ties);
@@ -479,12 +485,13 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const CachePara
     const int rank = scan_block(moved, warp_sum, total);
     if (threadIdx.x == 0) sh_moves = total;
     sync_blocks(blocks);
-    int hole = rank >> 16, tail = rank & 0xffff, moves = 0;
+    int hole = static_cast<int>(static_cast<uint32_t>(rank) >> 16), tail = rank & 0xffff, moves = 0;
     for (uint32_t r = 0; r < blocks; ++r) {
         const int c = cluster_load(&sh_moves, r);
-        hole += r < me ? c >> 16 : 0;
+        const int there = static_cast<int>(static_cast<uint32_t>(c) >> 16);
+        hole += r < me ? there : 0;
         tail += r < me ? c & 0xffff : 0;
-        moves += c >> 16;
+        moves += there;
     }
     int32_t* holes = p.holes + bh * p.half;
     int32_t* tails = p.tails + bh * p.half;
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(kAccThreads) accumulate_kernel(const CachePara
             for (int q = 0; q < q1; ++q) sum.add(to_float(w[q * p.wq]));
         }
     }
-    p.sums[bh * p.capacity + j] = sum.rounded();
+    p.sums[bh * p.sums_row + j] = sum.rounded();
 }
 
 __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const CacheParams p) {
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const CacheParams p)
     const int b = static_cast<int>(bh / p.heads);
     const int n = entries_of(p, b), m = min(n, p.budget);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float* sums = p.sums + bh * p.capacity;
+    const float* sums = p.sums + bh * p.sums_row;
     const int32_t* pos = p.pos + bh * p.capacity;
     float* out_acc = p.out_acc + bh * p.capacity;
     int32_t* out_pos = p.out_pos + bh * p.capacity;
@@ -649,17 +656,23 @@ __global__ void __launch_bounds__(256) move_kernel(const CacheParams p) {
 
 constexpr size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Blocks of a cluster: as few as hold the slots, but enough to fill the machine with
-// ranges of at least 1024 slots.  0: too long for eight.
+// Slots that each of n blocks holds, a multiple of four.
+int range_of(const mflat_cu_cache_t* c, int n) {
+    return (c->capacity / n + (c->capacity % n ? 1 : 0) + 3) & ~3;
+}
+
+// Blocks of a cluster: as few as hold the slots, sums and keys, but enough to fill the
+// machine with ranges of at least 1024 slots; eight hold twice as many keys alone.
+// 0: too long for that.
 int cluster_of(const mflat_cu_cache_t* c, int batch) {
     const int64_t bh = static_cast<int64_t>(batch) * c->heads;
     int n = 1;
-    auto range = [&] { return c->capacity / n + (c->capacity % n ? 1 : 0); };
-    while (n < kEvictCluster && (range() > kEvictSlots || (bh * n < 148 && range() >= 2048))) n *= 2;
-    return range() <= kEvictSlots ? n : 0;
+    while (n < kEvictCluster && (range_of(c, n) > kEvictSlots / 2 || (bh * n < 148 && range_of(c, n) >= 2048))) n *= 2;
+    return range_of(c, n) <= kEvictSlots ? n : 0;
 }
 
 struct CacheLayout {
+    bool out;                   // sums are in the workspace
     size_t holes, tails, tail_acc, tail_pos, sums, moves, end;
 };
 CacheLayout cache_layout(const mflat_cu_cache_t* c, int batch) {
@@ -670,9 +683,10 @@ CacheLayout cache_layout(const mflat_cu_cache_t* c, int batch) {
     l.tail_acc = l.tails + round256(half * 4);
     l.tail_pos = l.tail_acc + round256(half * 4);
     l.sums = l.tail_pos + round256(half * 4);
-    const bool is_long = cluster_of(c, batch) == 0;
-    l.moves = l.sums + (is_long ? round256(bh * c->capacity * 4) : 0);
-    l.end = l.moves + (is_long ? round256(bh * 4) : 0);
+    const int blocks = cluster_of(c, batch);
+    l.out = blocks == 0 || range_of(c, blocks) > kEvictSlots / 2;
+    l.moves = l.sums + (l.out ? round256(bh * ((static_cast<size_t>(c->capacity) + 3) & ~size_t(3)) * 4) : 0);
+    l.end = l.moves + (blocks == 0 ? round256(bh * 4) : 0);
     return l;
 }
 
@@ -699,7 +713,7 @@ int check_cache(const mflat_cu_cache_t* c, int batch) {
 template <class K>
 cudaError_t launch_evict(K kernel, int blocks, unsigned bh, size_t smem, cudaStream_t st, const CacheParams& p) {
     // always the same bound: calls from several threads may set it at once
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSlots * 8);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSlots * 4);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks), bh);
@@ -812,7 +826,8 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
     p.out_lens = out_lens;
     p.keys = c->key_bytes ? static_cast<char*>(keys) : nullptr;
     p.values = c->value_bytes ? static_cast<char*>(values) : nullptr;
-    p.sums = reinterpret_cast<float*>(w + l.sums);
+    p.sums = l.out ? reinterpret_cast<float*>(w + l.sums) : nullptr;
+    p.sums_row = (static_cast<int64_t>(c->capacity) + 3) & ~int64_t(3);
     p.holes = reinterpret_cast<int32_t*>(w + l.holes);
     p.tails = reinterpret_cast<int32_t*>(w + l.tails);
     p.moves = reinterpret_cast<int32_t*>(w + l.moves);
@@ -832,9 +847,9 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
     const unsigned bh = static_cast<unsigned>(batch * c->heads);
     const int blocks = cluster_of(c, batch);
     if (blocks > 0) {
-        p.range = (c->capacity / blocks + (c->capacity % blocks ? 1 : 0) + 3) & ~3;
+        p.range = range_of(c, blocks);
         CU_TRY(with_type(c->type, [&](auto zero) {
-            return launch_evict(evict_kernel<decltype(zero)>, blocks, bh, static_cast<size_t>(p.range) * 8, st, p);
+            return launch_evict(evict_kernel<decltype(zero)>, blocks, bh, static_cast<size_t>(p.range) * (l.out ? 4 : 8), st, p);
         }), "evict launch");
         return ST_OK;
     }

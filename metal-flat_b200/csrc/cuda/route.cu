@@ -17,10 +17,11 @@
 // cluster, which exchanges the counts in shared memory and scatters by itself.
 //
 // Bound by instructions: 16,384 tokens x 256 experts in 8 groups with a bias (16.8 MB,
-// 2.9 us at the copy rate) take 31.5 us, 25 of them in route_kernel at 0.7 instructions a
-// clock and scheduler; of a token's 925 instructions 265 load it and weigh its choice,
-// 95 find the floor, 135 list what reaches it, 135 rank that, 110 form the scores and 180
-// choose groups.  64 tokens take 8.9 us.
+// 2.9 us at the copy rate) take 33.5 us in the mean of 24 inputs (32 to 35: a cut that is
+// settled in 64 bits holds one block up by 2 us), 26 of them in route_kernel at 0.7
+// instructions a clock and scheduler; of a token's 925 instructions 265 load it and weigh
+// its choice, 95 find the floor, 135 list what reaches it, 135 rank that, 110 form the
+// scores and 180 choose groups.  64 tokens take 9.3 us.
 #include <cuda_runtime.h>
 
 #include <climits>

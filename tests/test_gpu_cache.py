@@ -229,13 +229,23 @@ def test_a_value_buffer_alone_and_none():
             assert torch.equal(v.cpu()[0, j, :20], values[0, j, at if vb else slice(0, 20)])
 
 
-@pytest.mark.parametrize("cap", [40_000, 150_001, 196_608, 196_609, 300_003])
+@pytest.mark.parametrize("cap", [40_000, 150_001, 196_608, 196_609, 300_003, 393_216, 393_217, 500_000])
 def test_long_caches(cap):
     g = gen(("long", cap))
     acc, pos, keys, values = make(g, 1, 2, cap, [cap - 3], dim=2)
     w = torch.rand(1, 2, 1, cap, generator=g)
     for budget in (100, cap // 2, cap - 4):
         check([cap - 3], [cap - 3], acc, pos, keys, values, budget, 10, 4, w)
+
+
+@pytest.mark.parametrize("cap", [196_608, 393_216, 400_000])
+def test_long_caches_whose_lower_half_leaves(cap):
+    """As many moves as there can be, all of a block's slots holes or tails."""
+    g = gen(("half", cap))
+    acc, pos, keys, values = make(g, 1, 1, cap, [cap], dim=2)
+    acc[:] = torch.arange(cap) / cap
+    check([cap], [cap], acc, pos, keys, values, cap // 2, 0, 0)
+    check([cap], [cap], -acc, pos, keys, values, cap // 2, 0, 0)
 
 
 def test_offsets_past_32_bits():
