@@ -6,7 +6,9 @@
 // hangs on the sums.  So each row first yields its k best logits (ties to the lower
 // token) and its sum from fp32 exponentials of a known error; the rows of a sequence
 // are merged by their keys (ties to the lower beam), and where two beams' keys come
-// closer than their errors those beams' sums are formed again from 64-bit terms.
+// closer than their errors those beams' sums are formed again from 64-bit terms, in an
+// order and about a reference (the row's largest logit) that the row's values alone
+// decide: equal rows get equal keys wherever they start.
 //
 // 64 x 8 rows of 128,000 bf16 logits (131 MB, 20.5 us for a plain read) take 33.4 us in the
 // row pass: 22.3 for loads and maxima, 4.4 for the exponentials (15 us of the special
@@ -480,13 +482,12 @@ template <class T>
 __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_constant__ BeamParams p) {
     __shared__ double sh_base[kMaxBeams];       // cum - log sum exp(x - ref); NaN: no candidates
     __shared__ double sh_ref[kMaxBeams];
-    __shared__ float sh_off[kMaxBeams];         // error of that
+    __shared__ float sh_off[kMaxBeams];         // error of that; 0: settled by the row's values alone
     __shared__ int sh_redo[kMaxBeams];
     __shared__ Choice list[kListMax];
     __shared__ Choice best[kMaxBeamK];
     __shared__ FloorShared sh_floor;
     __shared__ double sh_sum[kRowWarps];
-    __shared__ float sh_err;
     __shared__ int sh_n, sh_again;
     const int64_t b = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -536,9 +537,15 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         if (lane == 0) {
             sh_base[w] = base;
             sh_ref[w] = ref;
-            // exact beyond kWild (segment_exact's sums)
+            // beyond kWild segment_exact's sums: up to 2^22 64-bit additions in a row, in an
+            // order that hangs on where the row starts.  base and x - ref round by 2^-53 of
+            // themselves, at most 2^-52 (|base| + |key|) together (the key's part: error_of).
+            // A finished beam's key is its cum, and infinite logits only count.
             const bool fast = ref > -2.0 * kWild && ref < 2.0 * kWild;
-            sh_off[w] = fast ? sum_error(static_cast<float>(ref), p.vocab) : 0.0f;
+            const bool summed = ref > none && ref < -none;
+            sh_off[w] = !summed ? 0.0f
+                                : (fast ? sum_error(static_cast<float>(ref), p.vocab) : 1e-9f) +
+                                      0x1p-50f * static_cast<float>(fabs(base));
             sh_redo[w] = 0;
         }
     }
@@ -564,6 +571,9 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         else if (x == -neg_inf()) c.key = choice_key(base);
         return c;
     };
+    auto error_of = [&](const Choice& c) {
+        return sh_off[c.at >> 32] + 0x1p-51 * fabs(key_value(c.key));
+    };
     Choice own[kHeld];          // the held ones' keys, formed once an attempt
     auto form = [&] {
 #pragma unroll
@@ -581,31 +591,24 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
     };
     for (int attempt = 0; ; ++attempt) {
         __syncthreads();
-        if (warp == 0) {
-            float e = fmaxf(lane < p.beams ? sh_off[lane] : 0.0f, lane + 32 < p.beams ? sh_off[lane + 32] : 0.0f);
-            e = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(e)));
-            if (lane == 0) {
-                sh_n = 0;
-                sh_again = 0;
-                sh_err = 2.0f * e;
-            }
+        if (threadIdx.x == 0) {
+            sh_n = 0;
+            sh_again = 0;
         }
         form();
-        uint64_t mine = 0;
-        each([&](const Choice& c) { mine = c.key > mine ? c.key : mine; });
-        // a floor in fp32, rounded down, and lower by the sums' error: a key that much
-        // below could belong above
-        const uint32_t floor_f = block_floor(choice_key(__double2float_rd(key_value(mine))), p.k, p.rounds, sh_floor);
-        uint64_t floor_b = 1;
-        if (floor_f != 0u) floor_b = choice_key(static_cast<double>(key_value(floor_f)) - static_cast<double>(sh_err));
-        if (floor_b == 0) floor_b = 1;
-        if (mine >= floor_b) {
-            each([&](const Choice& c) {
-                if (c.key < floor_b) return;
-                const int at = shared_add(&sh_n, 1);
-                if (at < kListMax) list[at] = c;
-            });
-        }
+        // a floor under the k largest of the keys less their errors; a key that with its
+        // error stays below it cannot be among the k best
+        double mine = static_cast<double>(neg_inf());
+        each([&](const Choice& c) {
+            if (c.key != 0) mine = fmax(mine, key_value(c.key) - error_of(c));
+        });
+        const uint32_t floor_f = block_floor(choice_key(__double2float_rd(mine)), p.k, p.rounds, sh_floor);
+        const double floor_v = static_cast<double>(key_value(floor_f));
+        each([&](const Choice& c) {
+            if (c.key == 0 || key_value(c.key) + error_of(c) < floor_v) return;
+            const int at = shared_add(&sh_n, 1);
+            if (at < kListMax) list[at] = c;
+        });
         for (int j = threadIdx.x; j < p.k; j += kRowThreads) best[j] = Choice{0, 0};
         __syncthreads();
         const int n = min(sh_n, kListMax);
@@ -647,8 +650,8 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         auto close = [&](const Choice& x, const Choice& y) {
             const int u = static_cast<int>(x.at >> 32), w = static_cast<int>(y.at >> 32);
             if (x.key == 0 || y.key == 0 || u == w) return;
-            const double off = static_cast<double>(sh_off[u]) + sh_off[w];
-            if (off > 0.0 && !(key_value(x.key) - key_value(y.key) > off)) {
+            if (sh_off[u] == 0.0f && sh_off[w] == 0.0f) return;
+            if (!(key_value(x.key) - key_value(y.key) > error_of(x) + error_of(y))) {
                 sh_redo[u] = sh_redo[w] = 1;
                 sh_again = 1;
             }
@@ -669,7 +672,11 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
             if (sh_off[w] == 0.0f) continue;
             const int64_t r = b * p.beams + w;
             const T* row = static_cast<const T*>(p.logits) + r * p.stride;
-            const double m = sh_ref[w];
+            // the row's largest logit: the first of its segments' candidates
+            uint32_t top = 0;
+            for (int i = lane; i < p.splits; i += 32)
+                top = max(top, static_cast<uint32_t>(cand[(w * p.splits + i) * p.k] >> 32));
+            const double m = key_value(__reduce_max_sync(kFullMask, top));
             double sum = 0.0;
             for (int v = threadIdx.x; v < p.vocab; v += kRowThreads) {
                 const float x = to_float(row[v]);
@@ -684,6 +691,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
                 double all = 0.0;
                 for (int i = 0; i < kRowWarps; ++i) all += sh_sum[i];
                 sh_base[w] = static_cast<double>(p.cum[r]) - log(all);
+                sh_ref[w] = m;
                 sh_off[w] = 0.0f;
             }
         }

@@ -1,0 +1,76 @@
+"""Order of beams whose keys are equal, or equal up to roundings: rows that start at
+different offsets from a 16-byte boundary, logits of any size, cums of any size."""
+import numpy as np
+import pytest
+import torch
+
+import select_ref as R
+from test_gpu_beam import check, gen, select
+
+pytestmark = pytest.mark.gpu
+
+
+def equal_beams(b, w, row, cum):
+    """b sequences of w beams alike, from b rows of logits."""
+    x = row[:, None, :].expand(b, w, row.shape[1]).contiguous().cuda()
+    return x, torch.full((b, w), cum).cuda()
+
+
+def expect_equal_beams(x, cum, k):
+    """By logit, then beam, then token: what the rule leaves of equal rows and cums."""
+    out, _ = select(x, cum, k)
+    torch.cuda.synchronize()
+    w = x.shape[1]
+    for i, row in enumerate(R.f64(x[:, 0])):
+        token = np.tile(R.best(row, k), w)          # the lowest beams' k best hold all
+        beam = np.repeat(np.arange(w), k)
+        order = np.lexsort((token, beam, -row[token]))[:k]
+        np.testing.assert_array_equal(out[0][i].cpu().numpy(), beam[order])
+        np.testing.assert_array_equal(out[1][i].cpu().numpy(), token[order])
+
+
+# (an odd vocabulary: neighbouring rows start 4 bytes further from a boundary each)
+@pytest.mark.parametrize("size", [(64, 8, 50_257), (64, 4, 50_257), (16, 5, 50_001), (2, 4, 128_001), (40, 3, 9001)],
+                         ids=lambda s: "b%d_w%d_v%d" % s)
+@pytest.mark.parametrize("cum", [0.0, -7.3, -3e12])
+def test_equal_beams_at_different_offsets(size, cum):
+    b, w, v = size
+    g = gen(("offsets", size, cum))
+    # 16-bit values a step of 2^-6 apart: no two of them meet in 64 bits even at -3e12
+    row = (torch.randn(b, v, generator=g) * 64).round() / 64
+    for at in range(8192, v, 8192):     # larger ones where a row's offset moves the cuts
+        row[:, at - 2] = 4 + torch.rand(b, generator=g).mul(64).round() / 64
+    x, c = equal_beams(b, w, row, cum)
+    expect_equal_beams(x, c, 2 * w)
+
+
+@pytest.mark.parametrize("shift,spread", [(6e5, 4), (-6e5, 4), (3e7, 16)])
+def test_equal_beams_of_large_logits(shift, spread):
+    """Beyond the sizes that fp32 sums take.  Few terms weigh much, so that the last digits
+    of their sum reach the key."""
+    b, w, v = 64, 8, 50_257
+    row = spread * torch.randn(b, v, generator=gen(("large", shift))) + shift
+    x, c = equal_beams(b, w, row, 0.0)
+    expect_equal_beams(x, c, 16)
+
+
+def test_equal_beams_with_infinite_logits():
+    b, w, v = 4, 4, 9001
+    row = torch.randn(b, v, generator=gen("infinite"))
+    row[:, 77] = row[:, 4000] = row[:, 8999] = float("inf")
+    x, c = equal_beams(b, w, row, -2.0)
+    out, _ = select(x, c, 12)
+    # three a beam, with a third of the probability each
+    place = torch.arange(12)
+    assert torch.equal(out[0].cpu().long(), (place // 3).expand(b, 12))
+    assert torch.equal(out[1].cpu().long(), torch.tensor([77, 4000, 8999])[place % 3].expand(b, 12))
+
+
+@pytest.mark.parametrize("low", [-1e9, -1e30, -3.402823466e38])
+def test_first_step_with_the_other_beams_far_below(low):
+    """All beams alike and all but one out of the way: the usual first step."""
+    x = torch.randn(3, 1, 30_011, generator=gen(("first", low))).expand(3, 8, 30_011).contiguous().cuda()
+    cum = torch.full((3, 8), low)
+    cum[:, 2] = 0.0
+    out = check(x, cum.cuda(), 16)
+    assert (out[0].cpu() == 2).all()
