@@ -77,11 +77,14 @@ struct RouteParams {
 // the row's largest score: e 2.9e-7; the sum 2.4e-7 and, |x - m| weighted by the terms
 // averaging at most ln 1024 + 1, 1.1e-6, its additions 2^-24 each for a lane's experts
 // and 5 levels; reciprocal and product 1.8e-7.  Adding the bias rounds once more, 6e-8
-// of the result.
+// of the result, and so does a group's sum of two.
 __device__ __forceinline__ float tau_base(bool softmax, float largest, int per_lane) {
     return softmax ? 2.0f * (2.3e-6f + 6e-8f * per_lane) * largest : 5.4e-7f;
 }
 __device__ __forceinline__ float tau_of(float base, float c) { return base + 1.3e-7f * fabsf(c); }
+__device__ __forceinline__ float tau_of_two(float base, float a, float b) {
+    return tau_of(base, a) + tau_of(base, b) + 1.3e-7f * fabsf(a + b);
+}
 
 template <class S>
 __device__ __forceinline__ S exp_of(S v);
@@ -184,7 +187,7 @@ __device__ __forceinline__ S group_scores(const RouteParams& p, int lane, const 
         }
         const bool two = p.group_top == 2 && b != none;
         if (lane == g) mine = two ? a + b : a;
-        if (a != none) tau = fmaxf(tau, tau_of(base, float(a)) + (two ? tau_of(base, float(b)) : 0.0f));
+        if (a != none) tau = fmaxf(tau, two ? tau_of_two(base, float(a), float(b)) : tau_of(base, float(a)));
     }
     return mine;
 }
@@ -417,7 +420,7 @@ __device__ __forceinline__ bool choose_groups(const RouteParams& p, int lane, co
     const bool two = p.group_top == 2 && b > none;
     const float mine = two ? a + b : a;
     // all groups' largest; both terms are at least 0, so their bits order alike
-    float tau = a > none ? tau_of(base_tau, a) + (two ? tau_of(base_tau, b) : 0.0f) : 0.0f;
+    float tau = two ? tau_of_two(base_tau, a, b) : a > none ? tau_of(base_tau, a) : 0.0f;
     tau = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(tau)));
     if (exact) tau = 0.0f;
     const int base = (threadIdx.x & 31) - lane;
