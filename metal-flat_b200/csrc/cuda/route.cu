@@ -1058,16 +1058,17 @@ RoutePlan route_plan(const mflat_cu_router_t* r, int tokens) {
     RoutePlan l{};
     // a cluster's block keeps its choices in registers, one a thread
     const int threads = r->experts <= 256 ? 1024 : r->experts <= 512 ? 512 : 256;
-    l.tile = (tokens + kClusterTiles - 1) / kClusterTiles;
+    auto per = [tokens](int n) { return tokens / n + (tokens % n != 0); };      // up to 2^31 - 1 tokens
+    l.tile = per(kClusterTiles);
     if (tokens <= kClusterTokens && l.tile * r->k <= threads) {
         l.cluster = true;
         l.tiles = kClusterTiles;
         return l;
     }
     l.tiles = kTiles;
-    l.tile = (tokens + l.tiles - 1) / l.tiles;
+    l.tile = per(kTiles);
     if (l.tile > 65535) l.tile = 65535;
-    l.tiles = (tokens + l.tile - 1) / l.tile;
+    l.tiles = per(l.tile);
     auto round256 = [](size_t n) { return (n + 255) & ~size_t(255); };
     l.ranks = 0;
     l.counts = round256(static_cast<size_t>(tokens) * r->k * 2);
