@@ -351,7 +351,7 @@ MFLAT_API size_t mflat_cache_workspace_bytes(const mflat_cache_t*, int batch);
  * below the length are read.  d_rows (nullable): batch, valid query rows.  d_acc,
  * d_pos: batch x heads x capacity; outputs may be the same buffers.  Slots
  * behind the new length are left as they were in every output.  d_out_lens
- * (batch) must not be d_lens. */
+ * (batch) must not share memory with d_lens, d_seen or d_rows. */
 MFLAT_API mflat_status_t mflat_cache_evict_device(const mflat_cache_t*, int batch,
         const int32_t* d_lens, const int32_t* d_seen, const void* d_weights, int queries,
         const int64_t weight_stride[3], const int32_t* d_rows, const float* d_acc,

@@ -806,7 +806,10 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
         !aligned_to(out_pos, 4) || !aligned_to(out_lens, 4))
         return fail(ST_BAD_ARG, "misaligned pointer");
     if (batch == 0) return ST_OK;
-    if (out_lens == lens) return fail(ST_BAD_ARG, "out_lens must not be lens");
+    // one block writes a sequence's new length while its other heads' blocks still read these
+    for (const int32_t* in : {lens, seen, rows})
+        if (in && out_lens < in + batch && in < out_lens + batch)
+            return fail(ST_BAD_ARG, "out_lens must not share memory with lens, seen or rows");
     const CacheLayout l = cache_layout(c, batch);
     if (l.end > 0 && (!ws || ws_bytes < l.end || !aligned_to(ws, 256)))
         return fail(ST_BAD_ARG, "workspace missing, too small or not 256-byte aligned");

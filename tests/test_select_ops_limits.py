@@ -5,6 +5,20 @@ import pytest
 import mflat_b200 as M
 from test_select_ops_args import BAD, P, route, status
 
+NOWHERE = 10_000        # a device that is not there: a call that passes its checks ends at it
+
+
+def reasons(built_lib, fn, *a, **kw):
+    """What the log says of a refused call."""
+    seen = []
+    handler = M.LOG_HANDLER(lambda level, msg, user: seen.append(msg.decode()))
+    built_lib.mflat_set_log_handler(handler, None)
+    try:
+        status(fn, *a, **kw)
+    finally:
+        built_lib.mflat_set_log_handler(M.LOG_HANDLER(0), None)
+    return " ".join(seen)
+
 
 @pytest.mark.parametrize("experts", [2, 300])
 def test_router_workspace_up_to_the_last_token(built_lib, experts):
@@ -19,3 +33,15 @@ def test_router_workspace_up_to_the_last_token(built_lib, experts):
     for t in (1000, 148 * 65_535, 148 * 65_535 + 1, 2 ** 30, *(2 ** 31 - 1 - i for i in (0, 1, 7, 100, 146, 147, 148))):
         assert r.workspace_bytes(t) == need(t), t
         assert route(r, tokens=t, start=P, slots=P, ws=P, ws_bytes=need(t) - 1) == BAD
+
+
+@pytest.mark.parametrize("other", ["lens", "seen", "rows"])
+def test_new_lengths_apart_from_what_is_read(built_lib, other):
+    """A sequence's new length is written while its other heads still read the old ones."""
+    c = M.CacheEviction(2, 4, 100, 50, 16, 16, device=NOWHERE)
+    ok = dict(batch=3, lens=4 * P, seen=5 * P, rows=6 * P, acc=P, pos=P, keys=P, values=P, out_lens=2 * P, weights=P,
+              queries=1, ws=P, ws_bytes=1 << 30)
+    for at in (2 * P - 8, 2 * P, 2 * P + 8):
+        assert "out_lens" in reasons(built_lib, c.evict_device, **{**ok, other: at})
+    for at in (2 * P - 12, 2 * P + 12):         # next to it
+        assert "device" in reasons(built_lib, c.evict_device, **{**ok, other: at})
