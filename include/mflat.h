@@ -348,7 +348,8 @@ MFLAT_API size_t mflat_cache_workspace_bytes(const mflat_cache_t*, int batch);
 /* d_lens, d_seen: batch (entries held; tokens seen so far).  d_weights (nullable:
  * nothing to add): [b][heads * group][queries][slot], strides in elements from
  * sequence / head / query row to the next (NULL: rows of `capacity`); only slots
- * below the length are read.  d_rows (nullable): batch, valid query rows.  d_acc,
+ * below the length are read; group * queries at most 2^30, batch * heads at most
+ * 65,535.  d_rows (nullable): batch, valid query rows.  d_acc,
  * d_pos: batch x heads x capacity; outputs may be the same buffers.  Slots
  * behind the new length are left as they were in every output.  d_out_lens
  * (batch) must not share memory with d_lens, d_seen or d_rows. */

@@ -34,7 +34,7 @@ namespace {
 constexpr int kEvictThreads = 512, kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictSlots = 49152;      // keys a block holds, 4 bytes each; with half as many, sums too
 constexpr int kEvictCluster = 8;
-constexpr int kMaxCapacity = 1 << 30;
+constexpr int kMaxCapacity = 1 << 30, kMaxRows = 1 << 30;
 constexpr int kGather = 2048;           // keys of one digit that a block takes in
 constexpr int kAccThreads = 256;
 constexpr int kKeepThreads = 512, kKeepWarps = kKeepThreads / 32;
@@ -776,8 +776,9 @@ extern "C" int mflat_cu_cache_evict(const mflat_cu_cache_t* c, int batch, const 
                                     void* ws, size_t ws_bytes, int device, void* stream) {
     int rc = check_cache(c, batch);
     if (rc != ST_OK) return rc;
-    if (weights && (queries < 0 || static_cast<int64_t>(c->group) * queries > INT_MAX))
-        return fail(ST_BAD_ARG, "queries below 0, or group * queries of 2^31 or more");
+    // (the kernels count rows in steps of up to 32 past the last)
+    if (weights && (queries < 0 || static_cast<int64_t>(c->group) * queries > kMaxRows))
+        return fail(ST_BAD_ARG, "queries below 0, or group * queries above 2^30");
     CacheParams p{};
     p.heads = c->heads;
     p.group = c->group;

@@ -45,3 +45,14 @@ def test_new_lengths_apart_from_what_is_read(built_lib, other):
         assert "out_lens" in reasons(built_lib, c.evict_device, **{**ok, other: at})
     for at in (2 * P - 12, 2 * P + 12):         # next to it
         assert "device" in reasons(built_lib, c.evict_device, **{**ok, other: at})
+
+
+def test_more_rows_of_weights_than_the_kernels_count(built_lib):
+    """Row numbers stay below 2^31 in steps past the last row too."""
+    for group, queries, fits in [(1, 2 ** 30, True), (4, 2 ** 28, True), (1, 2 ** 30 + 1, False), (1, 2 ** 31 - 1, False),
+                                 (3, (2 ** 31 - 1) // 3, False), (2 ** 31 - 1, 1, False)]:
+        c = M.CacheEviction(1, group, 100, 50, 16, 16, device=NOWHERE)
+        # (strides of 0: all rows are one)
+        why = reasons(built_lib, c.evict_device, 1, P, P, P, P, P, P, 2 * P, weights=P, queries=queries,
+                      weight_stride=(0, 0, 0), ws=P, ws_bytes=1 << 30)
+        assert ("device" if fits else "queries") in why
