@@ -321,7 +321,7 @@ MFLAT_API mflat_status_t mflat_beam_select_device(const mflat_beam_t*, const voi
  * was, for every o < outer, b < batch, i < beams.  A row is `segments` pieces of
  * segment_bytes, segment_stride apart; strides in BYTES (0: dense), d_parents
  * rows parent_stride apart (0: beams).  Parents outside [0, beams) leave their
- * row alone; bytes between the pieces are not touched. */
+ * row alone; bytes between the pieces are not touched.  At most 65,535 sequences. */
 MFLAT_API mflat_status_t mflat_beam_reorder_device(void* d_states, const int32_t* d_parents,
         int64_t parent_stride, int outer, int batch, int beams, int segments,
         int64_t segment_bytes, int64_t segment_stride, int64_t row_stride, int64_t outer_stride,

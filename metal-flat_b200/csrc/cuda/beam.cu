@@ -757,8 +757,8 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const ReorderP
 template <class V>
 cudaError_t launch_reorder(const ReorderParams& p, cudaStream_t st) {
     const int64_t gx = (p.columns + kReorderThreads - 1) / kReorderThreads;
-    int outer = p.outer;
-    while (static_cast<int64_t>(outer) * p.batch > 65535) outer = (outer + 1) / 2;
+    int64_t outer = p.outer;            // up to 2^31 - 1
+    while (outer * p.batch > 65535) outer = (outer + 1) / 2;
     const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(outer * p.batch));
     if (p.beams <= 4) reorder_kernel<V, 4><<<grid, kReorderThreads, 0, st>>>(p);
     else if (p.beams <= 8) reorder_kernel<V, 8><<<grid, kReorderThreads, 0, st>>>(p);

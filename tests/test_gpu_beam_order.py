@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+import mflat_b200 as M
 import select_ref as R
 from test_gpu_beam import check, gen, select
 
@@ -106,3 +107,16 @@ def test_more_equal_keys_than_a_list_holds():
     out, _ = select(x.cuda(), torch.full((1, 64), -1e30).cuda(), 128)
     assert (out[0].cpu() == 0).all()
     np.testing.assert_array_equal(out[1][0].cpu().numpy(), R.best(R.f64(x[0, 0]), 128))
+
+
+def test_reorder_of_the_most_outer_rows():
+    """2^31 - 1 outer rows of two beams of a byte each."""
+    outer = 2 ** 31 - 1
+    x = torch.zeros(outer, 2, dtype=torch.uint8, device="cuda")
+    x[:, 1] = 7
+    x[::1001, 0] = 3
+    parents = torch.tensor([[1, 0]], dtype=torch.int32, device="cuda")
+    M.beam_reorder_device(x.data_ptr(), parents.data_ptr(), outer, 1, 2, 1)
+    torch.cuda.synchronize()
+    assert bool((x[:, 0] == 7).all())
+    assert bool((x[::1001, 1] == 3).all()) and int(torch.count_nonzero(x[:, 1])) == -(-outer // 1001)
