@@ -247,7 +247,8 @@ MFLAT_API mflat_flat_index_t* mflat_flat_load(const char* path, int device,
  * into CUDA graphs.  Scratch is the caller's `workspace` (256-byte aligned, the
  * size from *_workspace_bytes, no initial contents needed): calls that may
  * overlap on the GPU, and captured graphs that may, need one each.  Strides are
- * in elements unless they say bytes; 0 stands for densely packed rows.
+ * in elements unless they say bytes; 0 stands for densely packed rows, but among an
+ * eviction's weight_stride for rows that are the same.
  * A missing pointer -> NULL_ARG; a size, type or stride outside the stated
  * limits, a misaligned pointer (less than its element's size) or a workspace
  * too small -> BAD_ARG with a line in the log; CUDA failure -> DEVICE. */
@@ -312,7 +313,8 @@ typedef struct {
 MFLAT_API size_t mflat_beam_workspace_bytes(const mflat_beam_t*, int batch);
 /* d_logits: (batch * beams) rows of vocab; d_cum, d_finished (nullable): batch x
  * beams.  Outputs batch x k: parent beam, token, new cum; -1 / -1 / -inf padded.
- * d_out_scores may be d_cum where k = beams. */
+ * d_out_scores may be d_cum where k = beams.  A new cum is off by its rounding and at
+ * most 1.5e-6 + 8e-8 ln(vocab) + 2e-8 of the row's largest logit. */
 MFLAT_API mflat_status_t mflat_beam_select_device(const mflat_beam_t*, const void* d_logits,
         int64_t stride, const float* d_cum, const uint8_t* d_finished, int batch,
         int32_t* d_out_parents, int32_t* d_out_tokens, float* d_out_scores,
@@ -329,7 +331,7 @@ MFLAT_API mflat_status_t mflat_beam_reorder_device(void* d_states, const int32_t
 
 /* Eviction from a key/value cache by accumulated attention weight.  Per
  * sequence b and cache head h: acc' = acc + the weights of the group's query
- * heads and query rows, rounded once to fp32.  With more than `budget` entries
+ * heads and query rows, summed in about 48 bits and rounded to fp32.  With more than `budget` entries
  * the kept ones are those at positions < sink or >= seen[b] - recent (equals),
  * then the largest acc', ties to the lowest slot (NaN last).  The i-th free slot below
  * `budget` takes the i-th kept entry behind it: few rows move, slots lose the
@@ -347,7 +349,8 @@ typedef struct {
 MFLAT_API size_t mflat_cache_workspace_bytes(const mflat_cache_t*, int batch);
 /* d_lens, d_seen: batch (entries held; tokens seen so far).  d_weights (nullable:
  * nothing to add): [b][heads * group][queries][slot], strides in elements from
- * sequence / head / query row to the next (NULL: rows of `capacity`); only slots
+ * sequence / head / query row to the next (NULL: dense rows of `capacity`; a 0 in a
+ * stride that is given reads the same rows again: weights that heads share); only slots
  * below the length are read; group * queries at most 2^30, batch * heads at most
  * 65,535.  d_rows (nullable): batch, valid query rows.  d_acc,
  * d_pos: batch x heads x capacity; outputs may be the same buffers.  Slots

@@ -13,7 +13,19 @@
 // 64 x 8 rows of 128,000 bf16 logits (131 MB, 20.5 us for a plain read) take 33.4 us in the
 // row pass: 22.3 for loads and maxima, 4.4 for the exponentials (15 us of the special
 // function units, mostly beside the loads), 6.6 for floors, packs set aside and lists.
-// The merge adds 5 us of dependent exchanges, at any size.
+// The merge adds 5 to 6 us of dependent exchanges, at any size without close beams.
+//
+// Three paths are slower, and right for any values:
+// - Close beams: a sequence's one merge block reads their rows again, one by one, with a
+//   64-bit exponential a logit.  With one pair of equal beams among the 64 x 8 the call takes
+//   400 us, with all beams equal 2.3 ms (1 x 4 x 32,000: 86 and 159 us).  Random logits
+//   meet it rarely: none of 40 inputs of that size did (39.1 us, 39.4 at most).
+// - k above 32: the floor is the least of the warps' (k / 8)-th maxima, which many packs of
+//   a long segment reach.  Where they are more than kPackMax, it is read six times more
+//   (segment_exact): 64 x 8 x 128,000 take 50 us at k = 40, 300 at 48, 350 at 64 and 940 at
+//   128, 4 x 64 rows of that length 47, 755, 790 and 1400, 16 x 16 x 262,144 1.5 ms at 33.
+// - More candidates over the merge's floor than kListMax: every place is a pass over all
+//   of them.  1 x 64 x 50,257 take 26 us at k = 16, 180 at 96 and 3 ms at 128.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -712,7 +724,8 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
 // Reordering in place.  A thread owns the same bytes of all the rows of a
 // sequence: it reads every row that moves, then writes, so no other thread's
 // writes can come before its reads.  Bound by memory: 48 x 8 x 4 rows of 8 x 51 KB, about
-// 860 MB read and written, in 157 us (5.5 TB/s; a copy of all rows would move 1.3 GB).
+// 860 MB that move, in 157 us (5.5 TB/s; the counters see 930 MB, and a copy of all rows
+// would move 1.3 GB).  Rows of 33 to 64 beams spill 52 bytes of a thread's 255 registers.
 struct ReorderParams {
     char* states;
     const int32_t* parents;

@@ -1,7 +1,9 @@
 // cache.cu -- eviction from a key/value cache by accumulated attention weight.
 //
-// acc' = acc + the sum of the group's weights, formed in twice 24 bits and rounded
-// once, so that the kept set does not hang on an order of addition.  Of a cache over its
+// acc' = acc + the sum of the group's weights, formed in twice 24 bits and then rounded
+// to fp32: all but very rarely what the exact sum rounds to, so that the kept set all but
+// never hangs on an order of addition.  (The order is one of the call's sizes, strides and
+// alignment alone: equal calls give equal bits.)  Of a cache over its
 // budget m, the kept slots are the m largest of (protected, acc'), ties to the lower
 // slot: a radix select of the m-th key, then one ordered pass.  Slots of dropped
 // entries below m ("holes") take the kept entries at and behind m ("tails") in
@@ -156,7 +158,7 @@ __device__ __forceinline__ void sync_blocks(uint32_t blocks) {
 }
 
 // A sum as hi + lo: every addition to hi leaves its exact rounding error (Knuth's
-// two-sum), lo adds those up.
+// two-sum), lo adds those up, itself rounded at 2^-24 of its own, much smaller, value.
 struct TwoFloats {
     float hi, lo;
     __device__ __forceinline__ void add(float x) {

@@ -16,12 +16,17 @@
 // the order in which blocks run.  Up to kClusterTokens tokens the tiles' blocks are one
 // cluster, which exchanges the counts in shared memory and scatters by itself.
 //
-// Bound by instructions: 16,384 tokens x 256 experts in 8 groups with a bias (16.8 MB,
-// 2.9 us at the copy rate) take 33.5 us in the mean of 24 inputs (32 to 35: a cut that is
-// settled in 64 bits holds one block up by 2 us), 26 of them in route_kernel at 0.7
+// Bound by instructions: 16,384 tokens x 256 experts in 8 groups with a bias (18.4 MB with
+// the outputs, 2.9 us at the copy rate) take 33.7 us in the mean of 24 inputs (32 to 36: a
+// cut that is settled in 64 bits holds one block up by 2 us), 26 of them in route_kernel at 0.7
 // instructions a clock and scheduler; of a token's 925 instructions 265 load it and weigh
 // its choice, 95 find the floor, 135 list what reaches it, 135 rank that, 110 form the
 // scores and 180 choose groups.  64 tokens take 9.3 us.
+//
+// From k of about 29 on, more keys than a warp ranks (kCandMax) reach the floor of most
+// tokens, and those are chosen from 64-bit scores one expert at a time: 4096 x 256 take
+// 34.1 us at k = 28, 40.5 at 30 and 42.6 at 32.  512 experts with k = 32 take 75 us; 1024,
+// whose 32 experts a lane leave one block of 8 warps an SM, 34 us at k = 8 and 174 at 32.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -239,7 +244,9 @@ __device__ __forceinline__ void take_best(uint64_t (&key)[VPL], const float (&x)
 // Weights of the chosen experts: lane r holds the r-th one's logit.  Plain:
 // the score.  Renormalised: scores over their sum, formed from exponents relative
 // to the largest chosen logit (sigmoid: to min(that, 0)), so that scores too
-// small for fp32 still have their quotient.
+// small for fp32 still have their quotient.  In fp32 with the special function unit's
+// reciprocals: 7e-8 off in the mean where a single rounding would leave 3e-8.  Only the
+// choice needs more, and has it.
 __device__ __forceinline__ float weight_of(const RouteParams& p, bool chosen, float x, float m,
                                            float sum) {
     float w = 0.0f;
@@ -318,8 +325,9 @@ __device__ __forceinline__ void exact_keys(const RouteParams& p, const float (&x
 }
 
 // A token's kept groups in 64 bits, as bits; where a group is 2^n lanes, all bits of its
-// lanes alike.  The row is read again, so that the common path keeps its registers.
-// Every lane of the warp calls it.
+// lanes alike.  The row is read again, so that the common path need not keep it (at 256
+// experts that path spills 68 bytes of its 64 registers a thread as it is).  Every lane of
+// the warp calls it.
 template <class T, int LPT, int VPL>
 __device__ __noinline__ unsigned exact_groups(const RouteParams& p, int64_t t, int lane, bool live) {
     float x[VPL];
@@ -456,7 +464,7 @@ struct RouteScratch {
 };
 
 // The choice scores of a token's n candidates in 64 bits, lane l those of candidates
-// l and l + 32.  The row is read again, so that the common path keeps its registers.
+// l and l + 32.  The row is read again, so that the common path need not keep it.
 template <class T>
 __device__ __noinline__ void refine(const RouteParams& p, const T* row, const float2* cand, int n,
                                     double (&c)[2]) {
