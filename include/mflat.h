@@ -301,8 +301,8 @@ MFLAT_API mflat_status_t mflat_route_backward_device(const mflat_router_t*, cons
         void* d_out_grad, int64_t grad_stride, int device, void* stream);
 
 /* A beam search step over beams x vocabulary.  key = cum + log softmax(x)[v],
- * compared in 64 bits, a beam's own tokens by their logits; the k largest of a
- * sequence's beams * vocab, ties to the lowest beam, then token.  A finished beam proposes only (eos, cum); logits of
+ * compared in 64 bits; the k largest of a sequence's beams * vocab, ties to the
+ * lowest beam, then token.  A finished beam proposes only (eos, cum); logits of
  * -inf or NaN, and beams whose cum is not finite, propose nothing. */
 typedef struct {
     int beams, vocab, k;            /* 1..MAX_BEAMS; 1..2^30; 1..MAX_K              */

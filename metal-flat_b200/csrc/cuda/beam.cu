@@ -479,17 +479,12 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_segment_kernel(const __gr
     for (int j = n + threadIdx.x; j < p.k; j += kRowThreads) out[j] = 0;
 }
 
-// Equal keys of two beams go to the lower one.  A beam's own tokens always go by their
-// logits (`at` is a segment's candidate), which 64 bits of the key need not tell apart:
-// next to a cum of 1e12 they end at 1e-4.
 struct Choice {
     uint64_t key;       // choice_key of cum + log p in 64 bits
-    uint64_t at;        // logit key, ~token
-    int beam;
+    uint64_t at;        // beam, token
 };
 __device__ __forceinline__ bool better(const Choice& a, const Choice& b) {
-    if (a.key != b.key) return a.key > b.key;
-    return a.beam < b.beam || (a.beam == b.beam && a.at > b.at);
+    return a.key > b.key || (a.key == b.key && a.at < b.at);
 }
 
 // One sequence: its beams' sums, then the k best of the segments' candidates.  Few
@@ -567,35 +562,36 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         }
     }
     auto choice_of = [&](int i, uint64_t v) {
+        Choice c{0, 0};
         const int w = i / per_beam;
-        Choice c{0, 0, w};
         const double base = sh_base[w];
         if (base != base) return c;
+        c.at = static_cast<uint64_t>(w) << 32;
         if (p.finished && p.finished[b * p.beams + w]) {
             if (i == w * per_beam) {
                 c.key = choice_key(base);
-                c.at = 0xffffffffu - static_cast<uint32_t>(p.eos);
+                c.at |= static_cast<uint32_t>(p.eos);
             }
             return c;
         }
         const uint32_t key = static_cast<uint32_t>(v >> 32);
         if (key == 0u) return c;
         const float x = key_value(key);
-        c.at = v;
+        c.at |= 0xffffffffu - static_cast<uint32_t>(v);
         // +inf: only it counts, key = cum - log(how many)
         if (sh_ref[w] < static_cast<double>(-neg_inf())) c.key = choice_key(base + (static_cast<double>(x) - sh_ref[w]));
         else if (x == -neg_inf()) c.key = choice_key(base);
         return c;
     };
     auto error_of = [&](const Choice& c) {
-        return sh_off[c.beam] + 0x1p-51 * fabs(key_value(c.key));
+        return sh_off[c.at >> 32] + 0x1p-51 * fabs(key_value(c.key));
     };
     Choice own[kHeld];          // the held ones' keys, formed once an attempt
     auto form = [&] {
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
             const int i = j * kRowThreads + first;
-            own[j] = i < total ? choice_of(i, held[j]) : Choice{0, 0, 0};
+            own[j] = i < total ? choice_of(i, held[j]) : Choice{0, 0};
         }
     };
     // fn(choice) for every candidate of the thread
@@ -625,7 +621,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
             const int at = shared_add(&sh_n, 1);
             if (at < kListMax) list[at] = c;
         });
-        for (int j = threadIdx.x; j < p.k; j += kRowThreads) best[j] = Choice{0, 0, 0};
+        for (int j = threadIdx.x; j < p.k; j += kRowThreads) best[j] = Choice{0, 0};
         __syncthreads();
         const int n = min(sh_n, kListMax);
         if (sh_n <= kListMax) {
@@ -634,9 +630,9 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
             __syncthreads();
         } else {
             // more equal keys than the list holds: one block-wide best per place
-            Choice last{~0ull, 0, 0};
+            Choice last{~0ull, 0};
             for (int j = 0; j < p.k; ++j) {
-                Choice c{0, 0, 0};
+                Choice c{0, 0};
                 each([&](const Choice& x) {
                     if (x.key != 0 && better(last, x) && better(x, c)) c = x;
                 });
@@ -645,7 +641,6 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
                     Choice x;
                     x.key = __shfl_xor_sync(kFullMask, c.key, o);
                     x.at = __shfl_xor_sync(kFullMask, c.at, o);
-                    x.beam = __shfl_xor_sync(kFullMask, c.beam, o);
                     if (better(x, c)) c = x;
                 }
                 __syncthreads();
@@ -665,7 +660,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         // across its end: those beams' sums are formed again from 64-bit terms.
         const Choice last = best[p.k - 1];
         auto close = [&](const Choice& x, const Choice& y) {
-            const int u = x.beam, w = y.beam;
+            const int u = static_cast<int>(x.at >> 32), w = static_cast<int>(y.at >> 32);
             if (x.key == 0 || y.key == 0 || u == w) return;
             if (sh_off[u] == 0.0f && sh_off[w] == 0.0f) return;
             if (!(key_value(x.key) - key_value(y.key) > error_of(x) + error_of(y))) {
@@ -715,8 +710,8 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
     }
     for (int j = threadIdx.x; j < p.k; j += kRowThreads) {
         const Choice c = best[j];
-        p.parents[b * p.k + j] = c.key ? c.beam : -1;
-        p.tokens[b * p.k + j] = c.key ? static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(c.at)) : -1;
+        p.parents[b * p.k + j] = c.key ? static_cast<int32_t>(c.at >> 32) : -1;
+        p.tokens[b * p.k + j] = c.key ? static_cast<int32_t>(c.at & 0xffffffffu) : -1;
         p.scores[b * p.k + j] = static_cast<float>(key_value(c.key));
     }
 }

@@ -77,38 +77,6 @@ def test_first_step_with_the_other_beams_far_below(low):
     assert (out[0].cpu() == 2).all()
 
 
-@pytest.mark.parametrize("cum,scale", [(-1e12, 1e-3), (-1e15, 1.0), (-1e30, 1.0), (1e20, 1.0), (-5.0, 1e-18)])
-@pytest.mark.parametrize("v", [40, 30_011])
-def test_a_beams_tokens_go_by_their_logits(cum, scale, v):
-    """Also where its keys are equal in 64 bits; fewer choices are the first of more."""
-    b, w, k = 3, 4, 20
-    x = scale * torch.randn(b, w, v, generator=gen(("own", cum, scale, v)))
-    x[1, 1:] = x[1, :1]                         # one sequence of equal beams
-    c = torch.full((b, w), cum)
-    for beams in (1, w):
-        out, _ = select(x[:, :beams].contiguous().cuda(), c[:, :beams].contiguous().cuda(), k)
-        few, _ = select(x[:, :beams].contiguous().cuda(), c[:, :beams].contiguous().cuda(), 3)
-        torch.cuda.synchronize()
-        for i in range(b):
-            r = R.f64(x[i, :beams])
-            m = r.max(1, keepdims=True)
-            key = (np.float64(np.float32(cum)) - np.log(np.exp(r - m).sum(1, keepdims=True))) + (r - m)
-            beam, token = np.divmod(np.arange(beams * v), v)
-            order = np.lexsort((token, -r.ravel(), beam, -key.ravel()))[:k]
-            for got, want in zip(out, (beam, token)):
-                np.testing.assert_array_equal(got[i].cpu().numpy(), want[order])
-            for got, want in zip(few, (beam, token)):
-                np.testing.assert_array_equal(got[i].cpu().numpy(), want[order[:3]])
-
-
-def test_more_equal_keys_than_a_list_holds():
-    """64 equal beams of equal keys: the lowest beam's tokens, by their logits."""
-    x = torch.randn(1, 1, 40_009, generator=gen("many equal")).expand(1, 64, 40_009).contiguous()
-    out, _ = select(x.cuda(), torch.full((1, 64), -1e30).cuda(), 128)
-    assert (out[0].cpu() == 0).all()
-    np.testing.assert_array_equal(out[1][0].cpu().numpy(), R.best(R.f64(x[0, 0]), 128))
-
-
 def test_reorder_of_the_most_outer_rows():
     """2^31 - 1 outer rows of two beams of a byte each."""
     outer = 2 ** 31 - 1
