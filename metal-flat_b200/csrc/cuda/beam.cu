@@ -8,24 +8,28 @@
 // are merged by their keys (ties to the lower beam), and where two beams' keys come
 // closer than their errors those beams' sums are formed again from 64-bit terms, in an
 // order and about a reference (the row's largest logit) that the row's values alone
-// decide: equal rows get equal keys wherever they start.
+// decide: equal rows get equal keys wherever they start.  Next to a cum of 1e12, or
+// among logits of 1e-18, keys of different logits are equal too, and lists by logits
+// need not hold the lowest tokens of the last key: those come from whole rows.
 //
 // 64 x 8 rows of 128,000 bf16 logits (131 MB, 20.5 us for a plain read) take 33.4 us in the
 // row pass: 22.3 for loads and maxima, 4.4 for the exponentials (15 us of the special
 // function units, mostly beside the loads), 6.6 for floors, packs set aside and lists.
 // The merge adds 5 to 6 us of dependent exchanges, at any size without close beams.
 //
-// Three paths are slower, and right for any values:
+// These paths are slower, and right for any values:
 // - Close beams: a sequence's one merge block reads their rows again, one by one, with a
 //   64-bit exponential a logit.  With one pair of equal beams among the 64 x 8 the call takes
 //   400 us, with all beams equal 2.3 ms (1 x 4 x 32,000: 86 and 159 us).  Random logits
 //   meet it rarely: none of 40 inputs of that size did (39.1 us, 39.4 at most).
+// - Equal keys of different logits at the last place: the same second sum, then the rows
+//   from their start.  64 x 1 x 128,000 with a cum of -3.4e38 take 168 us for 15.
 // - k above 32: the floor is the least of the warps' (k / 8)-th maxima, which many packs of
 //   a long segment reach.  Where they are more than kPackMax, it is read six times more
 //   (segment_exact): 64 x 8 x 128,000 take 50 us at k = 40, 300 at 48, 350 at 64 and 940 at
 //   128, 4 x 64 rows of that length 47, 755, 790 and 1400, 16 x 16 x 262,144 1.5 ms at 33.
 // - More candidates over the merge's floor than kListMax: every place is a pass over all
-//   of them.  1 x 64 x 50,257 take 26 us at k = 16, 180 at 96 and 3 ms at 128.
+//   of them.  1 x 64 x 50,257 take 26 us at k = 16, 180 at 96 and 2.5 ms at 128.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -487,20 +491,115 @@ __device__ __forceinline__ bool better(const Choice& a, const Choice& b) {
     return a.key > b.key || (a.key == b.key && a.at < b.at);
 }
 
+// A sequence's beams in the merge.
+struct Beams {
+    double cum[kMaxBeams];      // NaN: no candidates
+    double log[kMaxBeams];      // log sum exp(x - ref)
+    double ref[kMaxBeams];      // -inf: finished
+    float off[kMaxBeams];       // error of the keys; 0: settled by the row's values alone
+    int redo[kMaxBeams];
+    int again, fill;
+
+    // where there are logits of +inf only they count, key = cum - log(how many)
+    __device__ __forceinline__ double key_of(int w, float x) const {
+        const double r = ref[w];
+        double d = static_cast<double>(x) - r;
+        if (r == static_cast<double>(-neg_inf())) d = x == -neg_inf() ? 0.0 : static_cast<double>(neg_inf());
+        return cum[w] + (d - log[w]);
+    }
+    __device__ __forceinline__ double error_of(const Choice& c) const {
+        return off[c.at >> 32] + 0x1p-51 * fabs(key_value(c.key));
+    }
+    // how far two keys of a beam can be off from one another by their roundings
+    __device__ __forceinline__ double rounding(int w, double key) const {
+        return 0x1p-48 * fabs(cum[w]) + 0x1p-49 * fabs(key);
+    }
+};
+
+// Neighbours in the order, x before y, that may be equal or the other way round.
+template <class T>
+__device__ __forceinline__ void beams_near(const BeamParams& p, Beams& sh, int64_t b, const Choice& x, const Choice& y) {
+    const int u = static_cast<int>(x.at >> 32), w = static_cast<int>(y.at >> 32);
+    if (x.key == 0 || y.key == 0 || (sh.off[u] == 0.0f && sh.off[w] == 0.0f)) return;
+    if (u == w) {
+        const T* row = static_cast<const T*>(p.logits) + (b * p.beams + u) * p.stride;
+        if (to_float(row[x.at & 0xffffffffu]) == to_float(row[y.at & 0xffffffffu])) return;
+    }
+    sh.redo[u] = sh.redo[w] = 1;
+    sh.again = 1;
+}
+
+// The thread's candidates that are their segments' k-th and reach the last key: if the
+// logits next to one give the same key, the segment may hold others of that key.
+template <class T>
+__device__ __forceinline__ void segments_full(const BeamParams& p, Beams& sh, const uint64_t* cand, int first, int total,
+                                           uint64_t last) {
+    constexpr uint32_t kStep = std::is_same_v<T, float> ? 1u : std::is_same_v<T, __half> ? 1u << 13 : 1u << 16;
+    for (int i = first; i < total; i += kRowThreads) {
+        const int w = i / (p.splits * p.k);
+        if (i % p.k != p.k - 1 || sh.cum[w] != sh.cum[w] || isinf(sh.ref[w])) continue;
+        const uint32_t at = static_cast<uint32_t>(cand[i] >> 32);
+        if (at == 0u) continue;
+        const double key = sh.key_of(w, key_value(at)), most = sh.off[w] == 0.0f ? 0.0 : sh.rounding(w, key);
+        if (choice_key(key) < last) continue;
+        if (!(key - sh.key_of(w, key_value(at - kStep)) <= most || sh.key_of(w, key_value(at + kStep)) - key <= most))
+            continue;
+        if (sh.off[w] == 0.0f) {
+            sh.fill = 1;
+        } else {
+            sh.redo[w] = 1;
+            sh.again = 1;
+        }
+    }
+}
+
+// The places of the last key, from the whole rows of the beams that have it (redo): beam
+// by beam, token by token.
+template <class T>
+__device__ __forceinline__ void fill_last_key(const BeamParams& p, const Beams& sh, int64_t b, Choice* best) {
+    __shared__ int hits[kRowWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t key = best[p.k - 1].key;
+    int filled = __syncthreads_count(threadIdx.x < p.k && best[threadIdx.x].key > key);
+    for (int w = 0; w < p.beams && filled < p.k; ++w) {
+        if (!sh.redo[w]) continue;
+        const uint64_t beam = static_cast<uint64_t>(w) << 32;
+        if (sh.ref[w] == static_cast<double>(neg_inf())) {
+            if (threadIdx.x == 0) best[filled] = Choice{key, beam | static_cast<uint32_t>(p.eos)};
+            ++filled;
+            continue;
+        }
+        const T* row = static_cast<const T*>(p.logits) + (b * p.beams + w) * p.stride;
+        for (int v0 = 0; v0 < p.vocab && filled < p.k; v0 += kRowThreads) {
+            const int v = v0 + threadIdx.x;
+            const float x = v < p.vocab ? to_float(row[v]) : neg_inf();
+            const bool hit = x > neg_inf() && choice_key(sh.key_of(w, x)) == key;
+            const unsigned who = __ballot_sync(kFullMask, hit);
+            __syncthreads();
+            if (lane == 0) hits[warp] = __popc(who);
+            __syncthreads();
+            int place = filled + __popc(who & ((1u << lane) - 1u));
+            for (int i = 0; i < kRowWarps; ++i) {
+                place += i < warp ? hits[i] : 0;
+                filled += hits[i];
+            }
+            if (hit && place < p.k) best[place] = Choice{key, beam | static_cast<uint32_t>(v)};
+        }
+    }
+    __syncthreads();
+}
+
 // One sequence: its beams' sums, then the k best of the segments' candidates.  Few
 // blocks run, so the time is the chain of loads and exchanges: all loads start
 // together, and the first kHeld candidates of a thread stay in registers.
 template <class T>
 __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_constant__ BeamParams p) {
-    __shared__ double sh_base[kMaxBeams];       // cum - log sum exp(x - ref); NaN: no candidates
-    __shared__ double sh_ref[kMaxBeams];
-    __shared__ float sh_off[kMaxBeams];         // error of that; 0: settled by the row's values alone
-    __shared__ int sh_redo[kMaxBeams];
+    __shared__ Beams sh;
     __shared__ Choice list[kListMax];
     __shared__ Choice best[kMaxBeamK];
     __shared__ FloorShared sh_floor;
     __shared__ double sh_sum[kRowWarps];
-    __shared__ int sh_n, sh_again;
+    __shared__ int sh_n;
     const int64_t b = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per_beam = p.splits * p.k, total = p.beams * per_beam;
@@ -510,6 +609,9 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
     // a warp takes every 8th candidate, of all beams: the floor is the better, the more
     // evenly the best ones lie over the warps
     const int first = lane * kRowWarps + warp;
+    uint32_t ends = 0;          // held ones that are their segments' k-th
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) ends |= (j * kRowThreads + first) % p.k == p.k - 1 ? 1u << j : 0u;
     grid_wait();
     uint64_t held[kHeld];
 #pragma unroll
@@ -527,7 +629,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         }
         const float cum = p.cum[r];
         const bool done = p.finished && p.finished[r];
-        double base = __longlong_as_double(0x7ff8000000000000ll), sum = 0.0;
+        double base = __longlong_as_double(0x7ff8000000000000ll), log_sum = 0.0, sum = 0.0;
         double ref = none;
         if (isfinite(cum) && !done) {       // else its segments wrote nothing
             ref = f;
@@ -542,34 +644,38 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
                 if (f > none) sum += f == ref ? part : part * exp(f - ref);
             }
             for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-            if (ref > none) base = static_cast<double>(cum) - log(sum);
+            if (ref > none) {
+                base = cum;
+                log_sum = log(sum);
+            }
         } else if (isfinite(cum)) {
             base = cum;
         }
         if (lane == 0) {
-            sh_base[w] = base;
-            sh_ref[w] = ref;
+            sh.cum[w] = base;
+            sh.log[w] = log_sum;
+            sh.ref[w] = ref;
             // beyond kWild segment_exact's sums: up to 2^22 64-bit additions in a row, in an
-            // order that hangs on where the row starts.  base and x - ref round by 2^-53 of
-            // themselves, at most 2^-52 (|base| + |key|) together (the key's part: error_of).
-            // A finished beam's key is its cum, and infinite logits only count.
+            // order that hangs on where the row starts.  A key's two differences and its sum
+            // round by 2^-53 of themselves, below 2^-51 (|cum| + |key|) together (error_of has
+            // the key's part).  A finished beam's key is its cum, and infinite logits only count.
             const bool fast = ref > -2.0 * kWild && ref < 2.0 * kWild;
             const bool summed = ref > none && ref < -none;
-            sh_off[w] = !summed ? 0.0f
+            sh.off[w] = !summed ? 0.0f
                                 : (fast ? sum_error(static_cast<float>(ref), p.vocab) : 1e-9f) +
-                                      0x1p-50f * static_cast<float>(fabs(base));
-            sh_redo[w] = 0;
+                                      0x1p-50f * fabsf(cum);
+            sh.redo[w] = 0;
         }
     }
     auto choice_of = [&](int i, uint64_t v) {
         Choice c{0, 0};
         const int w = i / per_beam;
-        const double base = sh_base[w];
-        if (base != base) return c;
+        const double cum = sh.cum[w];
+        if (cum != cum) return c;
         c.at = static_cast<uint64_t>(w) << 32;
         if (p.finished && p.finished[b * p.beams + w]) {
             if (i == w * per_beam) {
-                c.key = choice_key(base);
+                c.key = choice_key(cum);
                 c.at |= static_cast<uint32_t>(p.eos);
             }
             return c;
@@ -578,13 +684,8 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         if (key == 0u) return c;
         const float x = key_value(key);
         c.at |= 0xffffffffu - static_cast<uint32_t>(v);
-        // +inf: only it counts, key = cum - log(how many)
-        if (sh_ref[w] < static_cast<double>(-neg_inf())) c.key = choice_key(base + (static_cast<double>(x) - sh_ref[w]));
-        else if (x == -neg_inf()) c.key = choice_key(base);
+        c.key = choice_key(sh.key_of(w, x));
         return c;
-    };
-    auto error_of = [&](const Choice& c) {
-        return sh_off[c.at >> 32] + 0x1p-51 * fabs(key_value(c.key));
     };
     Choice own[kHeld];          // the held ones' keys, formed once an attempt
     auto form = [&] {
@@ -605,19 +706,20 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
         __syncthreads();
         if (threadIdx.x == 0) {
             sh_n = 0;
-            sh_again = 0;
+            sh.again = 0;
+            sh.fill = 0;
         }
         form();
         // a floor under the k largest of the keys less their errors; a key that with its
         // error stays below it cannot be among the k best
         double mine = static_cast<double>(neg_inf());
         each([&](const Choice& c) {
-            if (c.key != 0) mine = fmax(mine, key_value(c.key) - error_of(c));
+            if (c.key != 0) mine = fmax(mine, key_value(c.key) - sh.error_of(c));
         });
         const uint32_t floor_f = block_floor(choice_key(__double2float_rd(mine)), p.k, p.rounds, sh_floor);
         const double floor_v = static_cast<double>(key_value(floor_f));
         each([&](const Choice& c) {
-            if (c.key == 0 || key_value(c.key) + error_of(c) < floor_v) return;
+            if (c.key == 0 || key_value(c.key) + sh.error_of(c) < floor_v) return;
             const int at = shared_add(&sh_n, 1);
             if (at < kListMax) list[at] = c;
         });
@@ -655,33 +757,49 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
             }
             __syncthreads();
         }
-        if (attempt == 2) break;
         // Two beams' candidates closer than their sums' errors, in the selection or
-        // across its end: those beams' sums are formed again from 64-bit terms.
+        // across its end: those beams' sums are formed again from 64-bit terms.  So is one
+        // beam's, where keys of different logits are equal or nearly so, because next to
+        // a cum of 1e12 they end at 1e-4: which of them are equal hangs on the sum too.
         const Choice last = best[p.k - 1];
         auto close = [&](const Choice& x, const Choice& y) {
             const int u = static_cast<int>(x.at >> 32), w = static_cast<int>(y.at >> 32);
-            if (x.key == 0 || y.key == 0 || u == w) return;
-            if (sh_off[u] == 0.0f && sh_off[w] == 0.0f) return;
-            if (!(key_value(x.key) - key_value(y.key) > error_of(x) + error_of(y))) {
-                sh_redo[u] = sh_redo[w] = 1;
-                sh_again = 1;
+            const double kx = key_value(x.key), bound = u == w ? sh.rounding(u, kx) : sh.error_of(x) + sh.error_of(y);
+            // (a beam's keys this close come of equal logits, but for logits below 2^26 times
+            // the bound: larger ones lie further apart, those of fewer bits all the more)
+            return !(kx - key_value(y.key) > bound) &&
+                   !(u == w && fabs(kx - sh.cum[u] + sh.log[u] + sh.ref[u]) > 0x1p26 * bound);
+        };
+        // fn(x, y) for the pairs that decide
+        auto pairs = [&](auto&& fn) {
+            for (int j = threadIdx.x; j + 1 < p.k; j += kRowThreads) fn(best[j], best[j + 1]);
+            if (sh_n <= kListMax) {
+                for (int i = threadIdx.x; i < n; i += kRowThreads)
+                    if (better(last, list[i])) fn(last, list[i]);
+            } else {
+                each([&](const Choice& c) {
+                    if (better(last, c)) fn(last, c);
+                });
             }
         };
-        for (int j = threadIdx.x; j + 1 < p.k; j += kRowThreads) close(best[j], best[j + 1]);
-        if (sh_n <= kListMax) {
-            for (int i = threadIdx.x; i < n; i += kRowThreads)
-                if (better(last, list[i])) close(last, list[i]);
-        } else {
-            each([&](const Choice& c) {
-                if (better(last, c)) close(last, c);
-            });
-        }
+        bool doubt = false;
+        pairs([&](const Choice& x, const Choice& y) { doubt |= close(x, y); });
+        // A segment whose k candidates all reach the last key may hold others of that key,
+        // on lower tokens.
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) doubt |= ((ends >> j) & 1u) != 0u && last.key != 0 && own[j].key >= last.key;
+        for (int i = kHeld * kRowThreads + first; last.key != 0 && i < total; i += kRowThreads)
+            doubt |= i % p.k == p.k - 1 && choice_of(i, cand[i]).key >= last.key;
+        if (!__syncthreads_or(doubt)) break;
+        pairs([&](const Choice& x, const Choice& y) {
+            if (close(x, y)) beams_near<T>(p, sh, b, x, y);
+        });
+        if (last.key != 0) segments_full<T>(p, sh, cand, first, total, last.key);
         __syncthreads();
-        if (!sh_again) break;
+        if (!sh.again) break;           // (by the third attempt every sum has been formed again)
         for (int w = 0; w < p.beams; ++w) {
-            if (attempt == 0 && !sh_redo[w]) continue;
-            if (sh_off[w] == 0.0f) continue;
+            if (attempt == 0 && !sh.redo[w]) continue;
+            if (sh.off[w] == 0.0f) continue;
             const int64_t r = b * p.beams + w;
             const T* row = static_cast<const T*>(p.logits) + r * p.stride;
             // the row's largest logit: the first of its segments' candidates
@@ -702,11 +820,20 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
             if (threadIdx.x == 0) {
                 double all = 0.0;
                 for (int i = 0; i < kRowWarps; ++i) all += sh_sum[i];
-                sh_base[w] = static_cast<double>(p.cum[r]) - log(all);
-                sh_ref[w] = m;
-                sh_off[w] = 0.0f;
+                sh.log[w] = log(all);
+                sh.ref[w] = m;
+                sh.off[w] = 0.0f;
             }
         }
+    }
+    if (sh.fill) {
+        for (int w = threadIdx.x; w < p.beams; w += kRowThreads) sh.redo[w] = 0;
+        __syncthreads();
+        each([&](const Choice& c) {
+            if (c.key == best[p.k - 1].key) sh.redo[c.at >> 32] = 1;
+        });
+        __syncthreads();
+        fill_last_key<T>(p, sh, b, best);
     }
     for (int j = threadIdx.x; j < p.k; j += kRowThreads) {
         const Choice c = best[j];

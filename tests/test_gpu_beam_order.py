@@ -77,6 +77,65 @@ def test_first_step_with_the_other_beams_far_below(low):
     assert (out[0].cpu() == 2).all()
 
 
+LOW = -3.402823466e38
+
+
+@pytest.mark.parametrize("cum,scale", [(-1e12, 1e-3), (-1e15, 1.0), (-1e30, 1.0), (LOW, 3.0), (1e20, 1.0), (-5.0, 1e-18)])
+@pytest.mark.parametrize("v,kind", [(40, "fp32"), (30_011, "fp32"), (30_011, "bf16"), (9001, "fp16")])
+def test_keys_of_different_logits_that_are_equal_in_64_bits(cum, scale, v, kind):
+    """Ties go to the lowest beam, then token, whatever the logits are."""
+    if kind == "fp16":
+        scale = max(scale, 1e-3)
+    b, w = 4, 4
+    x = scale * torch.randn(b, w, v, generator=gen(("own", cum, scale, v)))
+    x[1, 1:] = x[1, :1]                         # a sequence of equal beams
+    x[2, 0, 7:] = -float("inf")                 # a beam that has fewer than are asked for
+    x[3, 1, ::2], x[3, 2] = float("nan"), 0.0
+    x = x.to(R.TYPES[kind])
+    c = torch.full((b, w), cum)
+    done = torch.zeros(b, w, dtype=torch.uint8)
+    done[0, 1] = done[2, 0] = done[3, 3] = 1
+    for beams, k in [(1, 1), (1, 3), (1, 20), (w, 3), (w, 20), (w, 128)]:
+        xs, cs, ds = (t[:, :beams].contiguous().cuda() for t in (x, c, done))
+        check(xs, cs, k)
+        check(xs, cs, k, ds, eos=v // 2)
+
+
+def test_beams_at_the_lowest_cum_fill_up():
+    """Few tokens allowed in the one beam that is alive: the others' fill the places."""
+    x = torch.full((2, 4, 20_003), -float("inf"))
+    x[:, 0, [5, 900]] = torch.tensor([1.0, 2.0])
+    x[:, 1:, 100:] = torch.randn(2, 3, 19_903, generator=gen("fill"))
+    cum = torch.full((2, 4), LOW)
+    cum[:, 0] = -1.0
+    out = check(x.cuda(), cum.cuda(), 8)
+    assert out[1][0].tolist() == [900, 5, 100, 101, 102, 103, 104, 105]
+
+
+def test_more_equal_keys_than_a_list_holds():
+    x = torch.randn(1, 1, 40_009, generator=gen("many equal")).expand(1, 64, 40_009).contiguous()
+    check(x.cuda(), torch.full((1, 64), -1e30).cuda(), 128)
+
+
+def test_zeros():
+    for v in (50, 20_011):
+        check(torch.zeros(2, 3, v).cuda(), torch.zeros(2, 3).cuda(), 9)
+        check(torch.zeros(2, 3, v).bfloat16().cuda(), torch.tensor([[0.0, 1.0, 1.0]] * 2).cuda(), 9)
+
+
+@pytest.mark.parametrize("v", [1, 2, 3, 30])
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_equal_beams_with_fewer_candidates_than_choices(v, kind):
+    for w, k in [(3, 3 * v + 1), (8, 128), (21, min(128, 21 * v))]:
+        g = gen(("few", v, kind, w))
+        x = (3 * torch.randn(6, 1, v, generator=g)).to(R.TYPES[kind]).expand(6, w, v).contiguous()
+        for shift in (0.0, -1e6, 53.3):
+            c = torch.randn(6, 1, generator=g).expand(6, w) + shift
+            check(x.cuda(), c.contiguous().cuda(), k)
+            done = (torch.rand(6, w, generator=g) < 0.3).to(torch.uint8)
+            check(x.cuda(), c.contiguous().cuda(), k, done.cuda(), eos=v - 1)
+
+
 def test_reorder_of_the_most_outer_rows():
     """2^31 - 1 outer rows of two beams of a byte each."""
     outer = 2 ** 31 - 1
