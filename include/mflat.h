@@ -331,11 +331,11 @@ MFLAT_API mflat_status_t mflat_beam_reorder_device(void* d_states, const int32_t
 
 /* Eviction from a key/value cache by accumulated attention weight.  Per
  * sequence b and cache head h: acc' = acc + the weights of the group's query
- * heads and query rows, summed in about 48 bits and rounded to fp32.  With more than `budget` entries
- * the kept ones are those at positions < sink or >= seen[b] - recent (equals),
- * then the largest acc', ties to the lowest slot (NaN last).  The i-th free slot below
- * `budget` takes the i-th kept entry behind it: few rows move, slots lose the
- * positions' order, d_pos tells them. */
+ * heads and query rows, summed in about 48 bits and rounded to fp32.  With more
+ * than `budget` entries the kept ones are those at positions < sink or >= seen[b] -
+ * recent (equals), then the largest acc', ties to the lowest slot (NaN last).  The
+ * i-th free slot below `budget` takes the i-th kept entry behind it: few rows move,
+ * slots lose the positions' order, d_pos tells them. */
 typedef struct {
     int heads, group;               /* cache heads; query heads per cache head      */
     int capacity;                   /* slots per (sequence, head), at most 2^30     */
@@ -352,10 +352,10 @@ MFLAT_API size_t mflat_cache_workspace_bytes(const mflat_cache_t*, int batch);
  * sequence / head / query row to the next (NULL: dense rows of `capacity`; a 0 in a
  * stride that is given reads the same rows again: weights that heads share); only slots
  * below the length are read; group * queries at most 2^30, batch * heads at most
- * 65,535.  d_rows (nullable): batch, valid query rows.  d_acc,
- * d_pos: batch x heads x capacity; outputs may be the same buffers.  Slots
- * behind the new length are left as they were in every output.  d_out_lens
- * (batch) must not share memory with d_lens, d_seen or d_rows. */
+ * 65,535.  d_rows (nullable): batch, valid query rows.  d_acc, d_pos: batch x heads x
+ * capacity; outputs may be the same buffers.  Slots behind the new length are left
+ * as they were in every output.  d_out_lens (batch) must not share memory with
+ * d_lens, d_seen or d_rows. */
 MFLAT_API mflat_status_t mflat_cache_evict_device(const mflat_cache_t*, int batch,
         const int32_t* d_lens, const int32_t* d_seen, const void* d_weights, int queries,
         const int64_t weight_stride[3], const int32_t* d_rows, const float* d_acc,

@@ -520,7 +520,7 @@ struct Beams {
 template <class T>
 __device__ __forceinline__ void beams_near(const BeamParams& p, Beams& sh, int64_t b, const Choice& x, const Choice& y) {
     const int u = static_cast<int>(x.at >> 32), w = static_cast<int>(y.at >> 32);
-    if (x.key == 0 || y.key == 0 || (sh.off[u] == 0.0f && sh.off[w] == 0.0f)) return;
+    if (sh.off[u] == 0.0f && sh.off[w] == 0.0f) return;
     if (u == w) {
         const T* row = static_cast<const T*>(p.logits) + (b * p.beams + u) * p.stride;
         if (to_float(row[x.at & 0xffffffffu]) == to_float(row[y.at & 0xffffffffu])) return;
@@ -533,7 +533,7 @@ __device__ __forceinline__ void beams_near(const BeamParams& p, Beams& sh, int64
 // logits next to one give the same key, the segment may hold others of that key.
 template <class T>
 __device__ __forceinline__ void segments_full(const BeamParams& p, Beams& sh, const uint64_t* cand, int first, int total,
-                                           uint64_t last) {
+                                              uint64_t last) {
     constexpr uint32_t kStep = std::is_same_v<T, float> ? 1u : std::is_same_v<T, __half> ? 1u << 13 : 1u << 16;
     for (int i = first; i < total; i += kRowThreads) {
         const int w = i / (p.splits * p.k);
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(kRowThreads) beam_merge_kernel(const __grid_co
             const double kx = key_value(x.key), bound = u == w ? sh.rounding(u, kx) : sh.error_of(x) + sh.error_of(y);
             // (a beam's keys this close come of equal logits, but for logits below 2^26 times
             // the bound: larger ones lie further apart, those of fewer bits all the more)
-            return !(kx - key_value(y.key) > bound) &&
+            return y.key != 0 && !(kx - key_value(y.key) > bound) &&
                    !(u == w && fabs(kx - sh.cum[u] + sh.log[u] + sh.ref[u]) > 0x1p26 * bound);
         };
         // fn(x, y) for the pairs that decide
